@@ -122,7 +122,7 @@ def draw(rng):
                       n_hi=n_hi, hq=hq, hkv=hkv, d=d, len_seed=len_seed)
     d = rng.choice([64, 128, 256])
     hq, hkv = rng.choice({64: [(14, 2), (16, 16)], 128: [(32, 8), (28, 4)], 256: [(16, 2), (8, 4)]}[d])
-    return _rope("", dtype=dtype, tokens=log(1, 16384 * 5120 // ((hq + 2 * hkv) * d)), hq=hq, hkv=hkv, d=d,
+    return _rope("", dtype=dtype, tokens=log(1, 15000 * 5120 // ((hq + 2 * hkv) * d)), hq=hq, hkv=hkv, d=d,
                  rot=rng.choice([d, d, d // 2, d // 4]), neox=rng.random() < 0.7, layout=rng.choice(["nhd", "hnd"]))
 
 
