@@ -121,7 +121,7 @@ def draw(rng):
         return _cross("", dtype=dtype, batch=batch, t_lo=max(1, t_hi // 8), t_hi=t_hi, n_lo=max(1, n_hi // 8),
                       n_hi=n_hi, hq=hq, hkv=hkv, d=d, len_seed=len_seed)
     d = rng.choice([64, 128, 256])
-    hq, hkv = rng.choice({64: [(14, 2), (16, 16)], 128: [(32, 8), (28, 4)], 256: [(16, 2), (8, 4)]}[d])
+    hq, hkv = rng.choice({64: [(14, 2), (12, 12)], 128: [(32, 8), (28, 4)], 256: [(16, 2), (8, 4)]}[d])
     return _rope("", dtype=dtype, tokens=log(1, 15000 * 5120 // ((hq + 2 * hkv) * d)), hq=hq, hkv=hkv, d=d,
                  rot=rng.choice([d, d, d // 2, d // 4]), neox=rng.random() < 0.7, layout=rng.choice(["nhd", "hnd"]))
 
