@@ -128,6 +128,76 @@ int vmc_paged_attention_decode(void* out, const void* query, const void* key_cac
                                int kv_format, int layout, int max_num_kv_splits,
                                void* workspace, size_t workspace_bytes, vmc_stream_t stream);
 
+/*
+ * Paged decode for a batch whose sequences share prefixes: one query token per
+ * sequence, semantics and page formats of vmc_paged_attention_decode, with the
+ * keys of a group's common prefix read once for the group instead of once per
+ * sequence.  No counterpart in the reference, whose block manager shares the
+ * prefix's blocks (src/memory/kv_cache_manager.cpp) while its decode reads
+ * them for each request.
+ *   out, query    [batch][num_heads][head_dim] of q_dtype; not overlapping
+ *   block_tables  int32 [batch][max_num_blocks_per_req]; entries < 0 are holes
+ *   seq_lens      int32 [batch], all tokens, the shared ones included; <= 0
+ *                 writes a zero row
+ *   group_starts  int32 [num_groups + 1], non-decreasing: group j holds the
+ *                 rows group_starts[j] .. group_starts[j+1] - 1; rows in no
+ *                 group share nothing.  May be NULL when num_groups is 0
+ *   shared_lens   int32 [num_groups]: tokens that a group's rows share, any
+ *                 number, not just whole pages.  A row of group j attends
+ *                 positions 0 .. min(shared_lens[j], seq_len) - 1 through the
+ *                 table row of the group's FIRST row, which has to list the
+ *                 pages of all shared_lens[j] tokens whatever that row's own
+ *                 length is, and the others through its own
+ *   workspace     >= vmc_shared_prefix_workspace_size(...) bytes, 16-byte
+ *                 aligned; calls that overlap on one workspace race
+ * Any block_size.  The group arrays are read on the device: a captured call
+ * follows their contents.  The size depends on the current device's CU count.
+ */
+size_t vmc_shared_prefix_workspace_size(int batch_size, int num_heads, int num_kv_heads,
+                                        int head_dim, int num_groups);
+int vmc_paged_attention_shared_prefix(void* out, const void* query, const void* key_cache,
+                                      const void* value_cache, const int32_t* block_tables,
+                                      const int32_t* seq_lens, const int32_t* group_starts,
+                                      const int32_t* shared_lens, int batch_size, int num_groups,
+                                      int num_heads, int num_kv_heads, int head_dim, int block_size,
+                                      int max_num_blocks_per_req, float scale, int q_dtype,
+                                      int kv_format, int layout, void* workspace,
+                                      size_t workspace_bytes, vmc_stream_t stream);
+
+/*
+ * Cross attention: decoder rows over an encoder's states of another length, no
+ * causal mask.  No counterpart in the reference (decoder-only models).
+ *   out           [num_tokens][num_heads][head_dim] of dtype, contiguous; not
+ *                 overlapping the inputs
+ *   query         value d of head h of token t at t * query_token_stride + h *
+ *                 query_head_stride + d (strides in values)
+ *   key, value    the states of all sequences, num_keys of them, strided the
+ *                 same way with heads 0 .. num_kv_heads - 1
+ *   query_starts  int32 [num_seqs + 1], non-decreasing: sequence s holds the
+ *                 tokens query_starts[s] .. query_starts[s+1] - 1.  Rows of no
+ *                 sequence (padding before the first and behind the last) are
+ *                 left as they are
+ *   key_starts, key_lens  int32 [num_seqs]: sequence s attends states
+ *                 key_starts[s] .. key_starts[s] + key_lens[s] - 1, cut to
+ *                 0 .. num_keys - 1; none: zero rows.  Sequences may overlap
+ *                 (share states), and lie packed or padded
+ *   workspace     >= vmc_cross_attention_workspace_size(...) bytes, 16-byte
+ *                 aligned; calls that overlap on one workspace race
+ * Strides are even and at least head_dim, key and value 4-byte aligned.  The
+ * starts and lengths are read on the device: a captured call follows their
+ * contents.  The size depends on the current device's CU count.
+ */
+size_t vmc_cross_attention_workspace_size(int num_tokens, int num_seqs, int num_heads,
+                                          int num_kv_heads, int head_dim);
+int vmc_cross_attention(void* out, const void* query, const void* key, const void* value,
+                        const int32_t* query_starts, const int32_t* key_starts,
+                        const int32_t* key_lens, int num_tokens, int num_keys, int num_seqs,
+                        int num_heads, int num_kv_heads, int head_dim, int64_t query_token_stride,
+                        int64_t query_head_stride, int64_t key_token_stride,
+                        int64_t key_head_stride, int64_t value_token_stride,
+                        int64_t value_head_stride, float scale, int dtype, void* workspace,
+                        size_t workspace_bytes, vmc_stream_t stream);
+
 /* ---- TurboQuant packed KV (src/cuda/turboquant_kernels.cu) ---- */
 
 /* Mirrors vm_c::TQConfig (include/vm_c/cuda/kernels_turboquant.h:10-75). */
@@ -272,6 +342,43 @@ int vmc_fused_qk_norm_rope_store(void* q_buf, void* k_buf, const void* v_buf,
                                  int is_neox, int64_t block_size, int64_t cache_stride,
                                  int kv_format, int layout, const vmc_tq_config* tq_config,
                                  int dtype, vmc_stream_t stream);
+
+/*
+ * RoPE and append from the fused QKV projection, one launch: Q rotated into
+ * query_out, K rotated into the paged cache (and / or key_out), V into the
+ * paged cache.  Beside vmc_fused_qk_norm_rope_store: any head_dim the attention
+ * entry points take, strided rows (slices of one projection), a rotation of
+ * part of the head, fp32 tables; no norm, and K makes no trip through HBM of
+ * its own.  No counterpart in the reference.
+ *   query, key, value  token t at t * *_token_stride values (num_heads or
+ *                 num_kv_heads heads of head_dim values, contiguous); 16-byte
+ *                 aligned, strides multiples of 8
+ *   query_out     [num_tokens][num_heads][head_dim]; may be query itself where
+ *                 that is contiguous, else not overlapping
+ *   key_out       [num_tokens][num_kv_heads][head_dim], or NULL; as query_out
+ *   cos_sin       float [max_position][rotary_dim], cos in [0, rotary_dim / 2),
+ *                 then sin; 16-byte aligned
+ *   position_ids  int64 [num_tokens]; a token whose position is outside
+ *                 [0, max_position) (padding) is skipped: its rows of
+ *                 query_out, key_out and the cache are left as they are
+ *   rotary_dim    a multiple of 16 up to head_dim; neox pairs (d, d +
+ *                 rotary_dim / 2), GPT-J pairs (2d, 2d + 1): a' = a cos - b sin,
+ *                 b' = b cos + a sin in fp32, rounded to dtype; the head's
+ *                 other values pass unchanged
+ *   key_cache     NULL: rotation only (key_out required, value unused).
+ *                 Otherwise K as rounded to dtype and V are appended at
+ *                 slot_mapping (int64, < 0 skips) as vmc_reshape_and_cache
+ *                 does: kv_format, layout, block_size, cache_stride as there
+ * For TurboQuant slots: key_out, then vmc_turboquant_store.
+ */
+int vmc_rope_and_cache(void* query_out, void* key_out, const void* query, const void* key,
+                       const void* value, const float* cos_sin, const int64_t* position_ids,
+                       void* key_cache, void* value_cache, const int64_t* slot_mapping,
+                       int num_tokens, int num_heads, int num_kv_heads, int head_dim,
+                       int rotary_dim, int64_t max_position, int64_t query_token_stride,
+                       int64_t key_token_stride, int64_t value_token_stride, int is_neox,
+                       int64_t block_size, int64_t cache_stride, int kv_format, int layout,
+                       int dtype, vmc_stream_t stream);
 
 /*
  * Split-KV paged decode over packed TurboQuant slots.

@@ -1,0 +1,49 @@
+"""Attention rows in 64 bits, with the error that a kernel's declared roundings
+allow each value.
+
+Weights w_k = softmax(s)_k, o = sum_k w_k v_k.  A score off by d_k changes o by
+sum_k w_k d_k (v_k - o) to first order, a V value off by a relative e_v by at
+most e_v sum_k w_k |v_k|, a weight off by a relative e_w by e_w sum_k w_k |v_k|
+in the numerator and e_w |o| through the sum.  The result is rounded once to the
+output type (half a step: eps / 2, relative).
+"""
+import numpy as np
+
+HALF_STEP = {"f16": 2.0 ** -11, "bf16": 2.0 ** -8}
+TINY = {"f16": 2.0 ** -25, "bf16": 2.0 ** -134}  # half the smallest subnormal
+
+
+def attend(q, k, v, scale, qt, e_k=0.0, e_v=0.0):
+    """q [d], k, v [n][d] in float64 -> (o [d], allowed error [d]).  e_k, e_v: relative
+    roundings of K and V values on their way into the products."""
+    d = q.shape[-1]
+    if len(k) == 0:
+        return np.zeros(d), np.zeros(d)
+    prod = k * q
+    s = prod.sum(1) * scale
+    w = np.exp(s - s.max())
+    w /= w.sum()
+    o = w @ v
+    # scores: fp32 sums of d products (any order: d roundings at most) and their
+    # scaling; the exponential, by base 2 with a rounded product, 2^-22 of |s| + 2
+    # roundings; relative roundings of K
+    size = np.abs(prod).sum(1) * abs(scale)
+    ds = size * ((d + 2) * 2.0 ** -24 + e_k) + np.abs(s - s.max()) * 2.0 ** -22 + 2.0 ** -22
+    # weights as two 16-bit terms of at least 8 bits each (2^-17), V's roundings, and
+    # fp32 sums over the keys, 64 at a time and their partial sums (2^-17 covers 128
+    # roundings in sequence: one a tile, rescales and the merge)
+    n_seq = 64 + 3 * (len(k) // 64 + 1) / 16
+    ew = 2.0 ** -17 + n_seq * 2.0 ** -24
+    av = w @ np.abs(v)
+    err = (w * ds) @ (np.abs(v) + np.abs(o)) + ew * (av + np.abs(o)) + e_v * av
+    err = err * 1.02  # second order
+    return o, err + (np.abs(o) + err) * HALF_STEP[qt] + TINY[qt]
+
+
+def check(got, want, err, what=""):
+    bad = ~(np.abs(got - want) <= err)
+    bad &= ~((got == want) | (np.isnan(got) & np.isnan(want)))
+    if bad.any():
+        i = tuple(np.argwhere(bad)[0])
+        raise AssertionError(f"{what}: {int(bad.sum())} of {bad.size} values off, first at {i}: "
+                             f"{got[i]} for {want[i]}, allowed {err[i]:.3g}")

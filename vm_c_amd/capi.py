@@ -94,6 +94,19 @@ def load():
     L.vmc_fused_qk_norm_rope_store.argtypes = [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I,
                                                _F, _I, _I64, _I64, _I, _I, C.POINTER(TQConfig), _I,
                                                _P]
+    L.vmc_rope_and_cache.restype = _I
+    L.vmc_rope_and_cache.argtypes = [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I64, _I64, _I64,
+                                     _I64, _I, _I64, _I64, _I, _I, _I, _P]
+    L.vmc_shared_prefix_workspace_size.restype = _SZ
+    L.vmc_shared_prefix_workspace_size.argtypes = [_I, _I, _I, _I, _I]
+    L.vmc_paged_attention_shared_prefix.restype = _I
+    L.vmc_paged_attention_shared_prefix.argtypes = [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F,
+                                                    _I, _I, _I, _P, _SZ, _P]
+    L.vmc_cross_attention_workspace_size.restype = _SZ
+    L.vmc_cross_attention_workspace_size.argtypes = [_I, _I, _I, _I, _I]
+    L.vmc_cross_attention.restype = _I
+    L.vmc_cross_attention.argtypes = [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I64, _I64, _I64, _I64,
+                                      _I64, _I64, _F, _I, _P, _SZ, _P]
     L.vmc_flash_attention_prefill.restype = _I
     L.vmc_flash_attention_prefill.argtypes = [_P, _P, _P, _P, _I, _I, _I, _I, _F, _P, _I, _P, _P,
                                               _P, _I64, _I, _I, _P]
@@ -361,6 +374,138 @@ def fused_qk_norm_rope_store(q, k, v, q_norm_weight, k_norm_weight, cos_sin_cach
         eps, int(bool(is_neox)), block_size, cache_stride, kv_format, layout,
         None if tq_cfg is None else C.byref(tq_cfg), _dtype_code(q), _stream(stream))
     _check(rc, "vmc_fused_qk_norm_rope_store")
+
+
+def _int32(what, n, **tensors):
+    """Index arrays of a call: contiguous int32 of n entries each."""
+    import torch
+    for name, t in tensors.items():
+        if t.dtype != torch.int32 or t.numel() != n or not t.is_contiguous():
+            raise VmcError(f"{what}: {name} is contiguous int32 [{n}]")
+
+
+def _on_current_device(t, what):
+    """A kernel runs on the current device: memory of another one is not its own."""
+    import torch
+    if t.device.type != "cuda" or t.device.index != torch.cuda.current_device():
+        raise VmcError(f"{what}: tensors are on {t.device}, not on the current device")
+
+
+def _token_stride(t, what):
+    """Values between the tokens of t [T][heads][dim], whose heads lie together."""
+    T, H, D = t.shape
+    st, sh, sd = t.stride()
+    if (sd != 1 and D > 1) or (sh != D and H > 1):
+        raise VmcError(f"{what}: the heads of a token have to be contiguous")
+    return st if T > 1 else H * D
+
+
+def rope_and_cache(query, key, value, cos_sin, position_ids, key_cache=None, value_cache=None, slot_mapping=None,
+                   block_size=16, query_out=None, key_out=None, is_neox=True, kv_format=KV_F16, layout=LAYOUT_NHD,
+                   cache_stride=0, stream=None):
+    """query [T][Hq][D], key, value [T][Hkv][D], slices of one projection's rows or
+    tensors of their own; cos_sin float [max_position][rotary_dim].  Rotates Q
+    into query_out (returned; allocated where it is None) and K into the paged
+    cache and / or key_out; appends V beside K."""
+    import torch
+    T, Hq, D = query.shape
+    Hkv = key.shape[1]
+    if key.shape != (T, Hkv, D) or (value is not None and value.shape != key.shape):
+        raise VmcError("rope_and_cache: query, key and value disagree in tokens, heads or head_dim")
+    if key.dtype != query.dtype or (value is not None and value.dtype != query.dtype):
+        raise VmcError("rope_and_cache: query, key and value have one dtype")
+    if cos_sin.dtype != torch.float32 or not cos_sin.is_contiguous():
+        raise VmcError("rope_and_cache: cos_sin is a contiguous float32 table")
+    for name, idx in (("position_ids", position_ids), ("slot_mapping", slot_mapping)):
+        if idx is not None and (idx.dtype != torch.int64 or idx.numel() != T or not idx.is_contiguous()):
+            raise VmcError(f"rope_and_cache: {name} is contiguous int64 [{T}]")
+    strides = (_token_stride(query, "query"), _token_stride(key, "key"),
+               0 if value is None else _token_stride(value, "value"))
+    for o, like in ((query_out, query), (key_out, key)):
+        if o is not None and (o.shape != like.shape or o.dtype != like.dtype or not o.is_contiguous()):
+            raise VmcError("rope_and_cache: query_out and key_out are contiguous, of their input's shape and dtype")
+    _on_current_device(query, "rope_and_cache")
+    if query_out is None:
+        query_out = torch.empty((T, Hq, D), dtype=query.dtype, device=query.device)
+        if stream is not None:
+            query_out.record_stream(stream)
+    rc = load().vmc_rope_and_cache(
+        _ptr(query_out), _ptr(key_out), _ptr(query), _ptr(key), _ptr(value), _ptr(cos_sin), _ptr(position_ids),
+        _ptr(key_cache), _ptr(value_cache), _ptr(slot_mapping), T, Hq, Hkv, D, cos_sin.shape[1], cos_sin.shape[0],
+        *strides, int(bool(is_neox)), block_size, cache_stride, kv_format, layout, _dtype_code(query), _stream(stream))
+    _check(rc, "vmc_rope_and_cache")
+    return query_out
+
+
+def shared_prefix_workspace_size(batch, num_heads, num_kv_heads, head_dim, num_groups):
+    return int(load().vmc_shared_prefix_workspace_size(batch, num_heads, num_kv_heads, head_dim, num_groups))
+
+
+def paged_attention_shared_prefix(out, query, key_cache, value_cache, block_tables, seq_lens, group_starts, shared_lens,
+                                  num_kv_heads, scale, block_size=16, kv_format=KV_F16, layout=LAYOUT_NHD,
+                                  workspace=None, stream=None):
+    """Paged decode of query [B][Hq][D]; group j is the rows group_starts[j] ..
+    group_starts[j + 1] - 1, whose first shared_lens[j] tokens are read once,
+    through the table row of its first row."""
+    B, Hq, D = query.shape
+    what = "paged_attention_shared_prefix"
+    num_groups = 0 if shared_lens is None else shared_lens.numel()
+    if num_groups:
+        _int32(what, num_groups, shared_lens=shared_lens)
+        _int32(what, num_groups + 1, group_starts=group_starts)
+    _int32(what, B, seq_lens=seq_lens)
+    _int32(what, B * block_tables.shape[1], block_tables=block_tables)
+    if out.shape != query.shape or out.dtype != query.dtype or not (out.is_contiguous() and query.is_contiguous()):
+        raise VmcError(f"{what}: query and out are contiguous, of one shape and dtype")
+    _on_current_device(query, what)
+    if workspace is None:
+        workspace = _workspace(max(1, shared_prefix_workspace_size(B, Hq, num_kv_heads, D, num_groups)), query, stream)
+    rc = load().vmc_paged_attention_shared_prefix(
+        _ptr(out), _ptr(query), _ptr(key_cache), _ptr(value_cache), _ptr(block_tables), _ptr(seq_lens),
+        _ptr(group_starts), _ptr(shared_lens), B, num_groups, Hq, num_kv_heads, D, block_size, block_tables.shape[1],
+        scale, _dtype_code(query), kv_format, layout, _ptr(workspace), workspace.numel() * workspace.element_size(),
+        _stream(stream))
+    _check(rc, "vmc_paged_attention_shared_prefix")
+    return out
+
+
+def cross_attention_workspace_size(num_tokens, num_seqs, num_heads, num_kv_heads, head_dim):
+    return int(load().vmc_cross_attention_workspace_size(num_tokens, num_seqs, num_heads, num_kv_heads, head_dim))
+
+
+def _strides(t, what):
+    """(values between tokens, values between heads) of t [N][heads][dim]."""
+    N, H, D = t.shape
+    st, sh, sd = t.stride()
+    if sd != 1 and D > 1:
+        raise VmcError(f"{what}: a head's values have to be contiguous")
+    return (st if N > 1 else H * D), (sh if H > 1 else D)
+
+
+def cross_attention(out, query, key, value, query_starts, key_starts, key_lens, scale, workspace=None, stream=None):
+    """query [T][Hq][D] over the states key, value [N][Hkv][D] (any token and head
+    strides): the tokens query_starts[s] .. query_starts[s + 1] - 1 attend states
+    key_starts[s] .. key_starts[s] + key_lens[s] - 1, no causal mask."""
+    T, Hq, D = query.shape
+    N, Hkv, _ = key.shape
+    S = key_lens.numel()
+    if key.shape != value.shape or key.shape[2] != D:
+        raise VmcError("cross_attention: query, key and value disagree in keys, heads or head_dim")
+    if not (query.dtype == key.dtype == value.dtype == out.dtype):
+        raise VmcError("cross_attention: query, key, value and out have one dtype")
+    _int32("cross_attention", S, key_starts=key_starts, key_lens=key_lens)
+    _int32("cross_attention", S + 1, query_starts=query_starts)
+    if out.shape != query.shape or not out.is_contiguous():
+        raise VmcError("cross_attention: out is contiguous and of query's shape")
+    strides = (*_strides(query, "query"), *_strides(key, "key"), *_strides(value, "value"))
+    _on_current_device(query, "cross_attention")
+    if workspace is None:
+        workspace = _workspace(max(1, cross_attention_workspace_size(T, S, Hq, Hkv, D)), query, stream)
+    rc = load().vmc_cross_attention(
+        _ptr(out), _ptr(query), _ptr(key), _ptr(value), _ptr(query_starts), _ptr(key_starts), _ptr(key_lens), T, N, S,
+        Hq, Hkv, D, *strides, scale, _dtype_code(query), _ptr(workspace), workspace.numel() * workspace.element_size(), _stream(stream))
+    _check(rc, "vmc_cross_attention")
+    return out
 
 
 def paged_attention_prefill(out, query, key_cache, value_cache, block_tables, token_to_seq,
