@@ -156,3 +156,19 @@ def test_ranges_are_cut(dev, d, t):
     c.k_lens.copy_(c.torch.tensor([20, 100, 9]))
     c.k0, c.n = np.array([0, 200, 0]), np.array([15, 10, 0])
     c.check()
+
+
+# so many items that each workgroup takes whole ones: sequences without rows or without
+# states, padding rows, a row block cut in the middle
+@pytest.mark.parametrize("d,heads", [(64, (32, 8)), (128, (32, 8)), (256, (16, 16))])
+@pytest.mark.parametrize("qt", ["f16", "bf16"])
+def test_whole_items(dev, d, heads, qt):
+    rng = np.random.default_rng(d)
+    n_seq = 130
+    t = rng.integers(30, 40, n_seq) if heads[0] > heads[1] else rng.integers(130, 150, n_seq)
+    n = rng.integers(1, 200, n_seq)
+    t[3], n[7] = 0, 0
+    t[40] = 1100
+    c = Cross(dev, t, n, heads, d, qt, seed=9, gap=(4, 5))
+    got = c.check(step=97)
+    assert (got[c.t_edges[7]:c.t_edges[8]] == 0).all()

@@ -8,6 +8,7 @@
 // of its sequence.  fp32 throughout (generic_row.hpp), rounded once.
 #include "generic_row.hpp"
 #include "shared_attn.hpp"
+#include "shared_plan.hpp"
 
 namespace vmc {
 namespace {
@@ -120,7 +121,7 @@ using namespace vmc;
 extern "C" size_t vmc_shared_prefix_workspace_size(int batch_size, int num_heads, int num_kv_heads, int head_dim,
                                                    int num_groups) {
     if (batch_size <= 0 || num_groups < 0 || !heads_valid(num_heads, num_kv_heads, head_dim)) return 0;
-    return 0;
+    return shared_tiles_workspace(true, batch_size, num_groups, num_heads, num_kv_heads, head_dim);
 }
 
 extern "C" int vmc_paged_attention_shared_prefix(void* out, const void* query, const void* key_cache,
@@ -148,6 +149,7 @@ extern "C" int vmc_paged_attention_shared_prefix(void* out, const void* query, c
         return VMC_EINVAL;
     if (workspace_bytes < vmc_shared_prefix_workspace_size(batch_size, num_heads, num_kv_heads, head_dim, num_groups))
         return VMC_ENOMEM;
+    if (!workspace || ((uintptr_t)workspace & 15) != 0) return VMC_EINVAL;
     SharedArgs a = {};
     a.out = reinterpret_cast<uint16_t*>(out);
     a.q = reinterpret_cast<const uint16_t*>(query);
@@ -171,14 +173,14 @@ extern "C" int vmc_paged_attention_shared_prefix(void* out, const void* query, c
     a.hnd = layout == VMC_LAYOUT_HND;
     a.bt = block_tables;
     a.seq_lens = seq_lens;
-    (void)workspace;
-    return shared_rows(a, reinterpret_cast<hipStream_t>(stream));
+    hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    return shared_tiles_take(a) ? shared_tiles(a, workspace, s) : shared_rows(a, s);
 }
 
 extern "C" size_t vmc_cross_attention_workspace_size(int num_tokens, int num_seqs, int num_heads, int num_kv_heads,
                                                      int head_dim) {
     if (num_tokens <= 0 || num_seqs <= 0 || !heads_valid(num_heads, num_kv_heads, head_dim)) return 0;
-    return 0;
+    return shared_tiles_workspace(false, num_tokens, num_seqs, num_heads, num_kv_heads, head_dim);
 }
 
 extern "C" int vmc_cross_attention(void* out, const void* query, const void* key, const void* value,
@@ -202,6 +204,7 @@ extern "C" int vmc_cross_attention(void* out, const void* query, const void* key
         return VMC_EINVAL;
     if (workspace_bytes < vmc_cross_attention_workspace_size(num_tokens, num_seqs, num_heads, num_kv_heads, head_dim))
         return VMC_ENOMEM;
+    if (!workspace || ((uintptr_t)workspace & 15) != 0) return VMC_EINVAL;
     SharedArgs a = {};
     a.out = reinterpret_cast<uint16_t*>(out);
     a.q = reinterpret_cast<const uint16_t*>(query);
@@ -225,6 +228,6 @@ extern "C" int vmc_cross_attention(void* out, const void* query, const void* key
     a.v_hs = value_head_stride;
     a.key_starts = key_starts;
     a.num_keys = num_keys;
-    (void)workspace;
-    return shared_rows(a, reinterpret_cast<hipStream_t>(stream));
+    hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    return shared_tiles_take(a) ? shared_tiles(a, workspace, s) : shared_rows(a, s);
 }

@@ -1,0 +1,118 @@
+// shared_plan.hpp -- the work axis of the shared-keys kernel (shared_tile.hpp): what
+// the plan kernel writes, how ranges of the axis map to workgroups and to partial
+// rows.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "shared_attn.hpp"
+
+namespace vmc {
+
+// One set of keys and the rows that attend them.  Paged calls: the groups' common
+// keys, then every row's own; contiguous calls: the sequences.
+struct SetDesc {
+    int row0, ntok;  // first row, rows (tokens); each stands for G query heads a KV head
+    int klo, khi;    // keys klo .. khi - 1 (tiles start at klo rounded down to 16)
+    int src;         // block-table row, or the key that key 0 is
+    int nb;          // items a KV head: ceil(ntok * G / rows of an item)
+    int tiles;       // 64-key tiles of an item
+    int own;         // paged: a row's own keys (else each row has seq_lens[row] at most)
+};
+
+struct PlanParams {
+    const int32_t* starts;
+    const int32_t* set_lens;
+    const int32_t* seq_lens;    // paged
+    const int32_t* key_starts;  // contiguous
+    int ns, rows;               // groups or sequences; rows
+    int nsets;                  // sets: ns (+ rows where paged)
+    int max_keys, num_keys;
+    int Hkv, G, RB;
+    int paged, whole;
+    int64_t* cum;   // [nsets + 1] units (whole: items) before each set
+    SetDesc* desc;  // [nsets]
+    int32_t* gs;    // [ns + 1] starts, cut to [0, rows] and made non-decreasing
+};
+
+struct TileParams {
+    uint16_t* out;
+    const uint16_t* q;
+    int64_t q_ts, q_hs;
+    int Hq, Hkv, G;
+    float scale;
+    const int64_t* cum;
+    const SetDesc* desc;
+    const int32_t* gs;
+    int ns, nsets, paged, whole;
+    int total_rows;
+    int grid, umin;  // ranges, and the fewest units of one
+    float* part;     // partial rows of D + 4 floats: o, m, l, two unused
+    const uint8_t* kp;
+    const uint8_t* vp;
+    int64_t k_row, k_head, v_row, v_head;  // bytes between keys (paged: of a page; v as k), between heads
+    int64_t page_bytes, max_blocks;
+    int bs;
+    const int32_t* bt;
+    const int32_t* seq_lens;
+};
+
+int shared_tile_d64(const TileParams& p, int src, bool q_bf16, int waves, unsigned grid, hipStream_t s);
+int shared_tile_d128(const TileParams& p, int src, bool q_bf16, int waves, unsigned grid, hipStream_t s);
+int shared_tile_d256(const TileParams& p, int src, bool q_bf16, int waves, unsigned grid, hipStream_t s);
+
+// The MFMA path of a call: whether it takes the shape, what workspace it needs (its
+// sizes alone decide), and the launches.
+bool shared_tiles_take(const SharedArgs& a);
+size_t shared_tiles_workspace(bool paged, int rows, int nsets, int Hq, int Hkv, int D);
+int shared_tiles(const SharedArgs& a, void* ws, hipStream_t s);
+
+namespace {
+
+// ranges that a total of units is cut into
+__host__ __device__ __forceinline__ int plan_ranges(int64_t total, int grid, int umin) {
+    const int64_t n = (total + umin - 1) / umin;
+    return (int)(n < grid ? n : grid);
+}
+
+// the range that holds unit u of total, ranges w being [w total / n, (w + 1) total / n)
+__device__ __forceinline__ int plan_range_of(int64_t u, int64_t total, int n) {
+    return (int)(((u + 1) * n - 1) / total);
+}
+
+// last s in [0, n) with cum[s] <= u (cum non-decreasing, cum[0] <= u); one wave, 64
+// probes a round
+template <typename T>
+__device__ __forceinline__ int plan_find(const T* cum, int n, int64_t u, int lane) {
+    int lo = 0, len = n;
+    while (len > 1) {
+        const int step = (len + 63) / 64;
+        const int64_t at = (int64_t)lane * step;
+        const bool in = at < len && (int64_t)cum[lo + (at < len ? at : 0)] <= u;
+        const int k = __popcll(__ballot(in)) - 1;
+        lo += max(k, 0) * step;
+        len = min(step, len - max(k, 0) * step);
+    }
+    return __builtin_amdgcn_readfirstlane(lo);
+}
+
+// First partial row of the piece of item (g, rb) of set d in a range.  Pieces follow
+// the axis, where each step goes to the next item or the next range: range *
+// rb_rows + (rows of the items before) grows by at least a piece's rows with
+// each step.  grid * rb_rows + 2 * rows * Hq rows in all.
+__device__ __forceinline__ int64_t plan_rows_paged(int range, int rb_rows, int Hq, int G, int rows, const SetDesc& d,
+                                                   int g, int rb) {
+    return (int64_t)range * rb_rows + (int64_t)Hq * ((d.own ? rows : 0) + (int64_t)d.row0) + (int64_t)g * d.ntok * G +
+           rb * rb_rows;
+}
+
+// Contiguous calls write whole items directly: a range has two cut ones at most, one
+// that began before it and one that goes on behind it
+__device__ __forceinline__ int64_t plan_rows_local(int range, int rb_rows, bool began_before) {
+    return (2 * (int64_t)range + (began_before ? 0 : 1)) * rb_rows;
+}
+
+}  // namespace
+}  // namespace vmc

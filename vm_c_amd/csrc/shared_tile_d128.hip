@@ -1,0 +1,10 @@
+// shared_tile_d128.hip -- the shared-keys MFMA kernel (shared_tile.hpp) at head_dim 128.
+#include "shared_tile.hpp"
+
+namespace vmc {
+
+int shared_tile_d128(const TileParams& p, int src, bool q_bf16, int waves, unsigned grid, hipStream_t s) {
+    return dispatch_tile<128>(p, src, q_bf16, waves, grid, s);
+}
+
+}  // namespace vmc
