@@ -13,9 +13,10 @@ HALF_STEP = {"f16": 2.0 ** -11, "bf16": 2.0 ** -8}
 TINY = {"f16": 2.0 ** -25, "bf16": 2.0 ** -134}  # half the smallest subnormal
 
 
-def attend(q, k, v, scale, qt, e_k=0.0, e_v=0.0):
+def attend(q, k, v, scale, qt, e_k=0.0, e_v=0.0, mixed=False):
     """q [d], k, v [n][d] in float64 -> (o [d], allowed error [d]).  e_k, e_v: relative
-    roundings of K and V values on their way into the products."""
+    roundings of K and V values on their way into the products; mixed: bf16 V whose
+    chunks of 16 keys differ in size."""
     d = q.shape[-1]
     if len(k) == 0:
         return np.zeros(d), np.zeros(d)
@@ -29,13 +30,25 @@ def attend(q, k, v, scale, qt, e_k=0.0, e_v=0.0):
     # roundings; relative roundings of K
     size = np.abs(prod).sum(1) * abs(scale)
     ds = size * ((d + 2) * 2.0 ** -24 + e_k) + np.abs(s - s.max()) * 2.0 ** -22 + 2.0 ** -22
-    # weights as two 16-bit terms of at least 8 bits each (2^-17), V's roundings, and
-    # fp32 sums over the keys, 64 at a time and their partial sums (2^-17 covers 128
-    # roundings in sequence: one a tile, rescales and the merge)
+    # fp32 sums over the keys, 64 at a time, and of their partial results: n_seq
+    # roundings in sequence
     n_seq = 64 + 3 * (len(k) // 64 + 1) / 16
-    ew = 2.0 ** -17 + n_seq * 2.0 ** -24
+    es = n_seq * 2.0 ** -24
+    # weights on their way into the products with V (the sum of the weights takes them
+    # unrounded): for a bf16 result one fp16 term, half a step of which is 2^-11; for
+    # an fp16 result two terms, of which a first bf16 one leaves 2^-8 and a second
+    # half a step of its own binade, 2^-17 of the weight
+    ew = 2.0 ** -11 if qt == "bf16" else 2.0 ** -17
     av = w @ np.abs(v)
-    err = (w * ds) @ (np.abs(v) + np.abs(o)) + ew * (av + np.abs(o)) + e_v * av
+    err = (w * ds) @ (np.abs(v) + np.abs(o)) + es * (av + np.abs(o)) + (ew + e_v) * av
+    # bf16 V as fp16, 16 keys by a power of two: off by 2^-25 over the scale, which is 2^8,
+    # or 1 beside values of 256 and more.  Weights of 2^-32 of the largest and less meet
+    # the end of fp16, 2^20 earlier where a chunk is scaled that much more than another
+    if qt == "bf16":
+        err = err + 2.0 ** (-25 if mixed else -33)
+        if mixed:
+            err = err + 2.0 ** -12 * w.max() * np.abs(v * (np.abs(v).max(1, keepdims=True) < 2.0 ** -12)).sum(0)
+            err = err + 2.0 ** -24 * w.max() * np.abs(v).sum(0)
     err = err * 1.02  # second order
     return o, err + (np.abs(o) + err) * HALF_STEP[qt] + TINY[qt]
 

@@ -54,7 +54,7 @@ class Cross:
         return self.capi.cross_attention(out, self.q, self.k, self.v, self.starts, self.k_starts, self.k_lens,
                                          self.scale, workspace=workspace, stream=stream)
 
-    def want(self, step=1):
+    def want(self, step=1, mixed=False):
         q, k, v = (x.cpu().double().numpy() for x in (self.q, self.k, self.v))
         o, err = np.full(q.shape, 7.0), np.zeros(q.shape)  # rows of no sequence stay
         seen = np.zeros(len(q), bool)
@@ -67,12 +67,13 @@ class Cross:
                 seen[r] = True
                 for h in range(self.hq):
                     g = h // (self.hq // self.hkv)
-                    o[r, h], err[r, h] = attend(q[r, h], k[at, g], v[at, g], self.scale, self.qt)
+                    o[r, h], err[r, h] = attend(q[r, h], k[at, g], v[at, g], self.scale, self.qt,
+                                                  mixed=mixed)
         return o, err, seen
 
-    def check(self, got=None, step=1):
+    def check(self, got=None, step=1, mixed=False):
         got = (self.run() if got is None else got).cpu().double().numpy()
-        o, err, seen = self.want(step)
+        o, err, seen = self.want(step, mixed)
         check(got[seen], o[seen], err[seen])
         return got
 
@@ -172,3 +173,26 @@ def test_whole_items(dev, d, heads, qt):
     c = Cross(dev, t, n, heads, d, qt, seed=9, gap=(4, 5))
     got = c.check(step=97)
     assert (got[c.t_edges[7]:c.t_edges[8]] == 0).all()
+
+
+# V of any magnitude: all values of a size, single outliers, one dim far from the others,
+# chunks of 16 keys of different sizes, values that no 16-bit scale fits
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("t", [3, 70])
+@pytest.mark.parametrize("size", ["300", "7e4", "1e30", "1e-5", "1e-12", "1e-30", "outlier", "dim", "chunks", "zeros"])
+def test_value_magnitudes(dev, d, t, size):
+    def edit(c, k, v):
+        if size == "outlier":
+            v[77, 0, 5] = 3e4
+            v[150, 1, 9] = 1e6
+        elif size == "dim":
+            v[..., 7] *= 1e-4
+            v[..., 8] *= 1e3
+        elif size == "chunks":
+            v *= np.repeat([1, 1e-6, 700, 1e-3, 1, 9e4, 1e-9], 32)[:200, None, None]
+        elif size == "zeros":
+            v[16:80] = 0
+            v[100:] = 0
+        else:
+            v *= float(size)
+    Cross(dev, [t, t], [130, 70], (8, 2), d, "bf16", seed=10, edit=edit).check(mixed=True)

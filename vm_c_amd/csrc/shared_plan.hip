@@ -15,207 +15,393 @@ namespace vmc {
 namespace {
 
 constexpr int kPlanThreads = 1024;
+constexpr int kUnitsMin = kItemCost + 1;  // fewest units of a range: one tile
+constexpr int kPlanCached = 1024;  // sets that the plan keeps in LDS
 
-template <typename T, typename Op>
-__device__ __forceinline__ T block_incl_scan(T v, T* sh, Op op, T* total) {
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+// Inclusive scan over the workgroup of N values a thread by op; all: the last one's.
+template <int N, typename T, typename Op>
+__device__ __forceinline__ void block_incl_scan(T (&v)[N], T (*sh)[N], Op op, T (&all)[N]) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, nw = blockDim.x >> 6;
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const T o = __shfl_up(v, d, kWave);
-        if (lane >= d) v = op(v, o);
-    }
-    if (lane == 63) sh[w] = v;
-    __syncthreads();
-    T all = sh[0];
-    T before = sh[0];
+    for (int d = 1; d < 64; d <<= 1)
 #pragma unroll
-    for (int i = 1; i < kPlanThreads / 64; ++i) {
-        if (i < w) before = op(before, sh[i]);
-        all = op(all, sh[i]);
-    }
-    if (w > 0) v = op(before, v);
-    *total = all;
+        for (int k = 0; k < N; ++k) {
+            const T o = __shfl_up(v[k], d, kWave);
+            if (lane >= d) v[k] = op(v[k], o);
+        }
+    if (lane == 63)
+#pragma unroll
+        for (int k = 0; k < N; ++k) sh[w][k] = v[k];
     __syncthreads();
-    return v;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        T run = sh[0][k], before = run;
+        for (int i = 1; i < nw; ++i) {
+            if (i == w) before = run;
+            run = op(run, sh[i][k]);
+        }
+        if (w > 0) v[k] = op(before, v[k]);
+        all[k] = run;
+    }
+    __syncthreads();
 }
 
+__device__ __forceinline__ int64_t div_small(int64_t x, int64_t y) {  // x, y >= 0; y > 0
+    return ((x | y) >> 32) == 0 ? (int64_t)((uint32_t)x / (uint32_t)y) : x / y;
+}
+
+// tiles before unit u of a set (with the first tile's place at or after u in *rec)
+__device__ __forceinline__ int64_t tiles_before(const SetDesc& d, int64_t cum, int64_t cumt, int64_t u, RangeRec* rec) {
+    const int64_t rem = u - cum;
+    const int per = d.tiles + kItemCost;
+    const int64_t item = div_small(rem, per);
+    const int x = max((int)(rem - item * per) - kItemCost, 0);
+    if (rec) {
+        rec->g = (int)div_small(item, d.nb);
+        rec->rb = (int)(item - (int64_t)rec->g * d.nb);
+        rec->t = x;
+    }
+    return cumt + item * d.tiles + x;
+}
+
+// CACHED: the sets fit the LDS copies, which later steps of the plan read instead of
+// what it has just written
+template <bool CACHED>
 __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(PlanParams p) {
-    __shared__ int shi[kPlanThreads / 64];
-    __shared__ long long shl[kPlanThreads / 64];
-    const int tid = threadIdx.x;
+    constexpr int NC = CACHED ? kPlanCached : 1;
+    __shared__ int shi[kPlanThreads / 64][1];
+    __shared__ long long shl[kPlanThreads / 64][2];
+    __shared__ long long s_cum[NC + 1], s_cumt[NC + 1];
+    __shared__ SetDesc s_desc[NC];
+    __shared__ int s_gs[NC + 1];
+    const int tid = threadIdx.x, nt = blockDim.x;
+    // lengths of this thread's first set: on their way while the starts are scanned
+    int len = 0, key0 = 0;
+    auto lengths = [&](int i) {
+        if (i < p.ns) {
+            len = p.set_lens[i];
+            if (!p.paged) key0 = p.key_starts[i];
+        } else if (i < p.nsets) {
+            len = p.seq_lens[i - p.ns];
+        }
+    };
+    lengths(tid);
     int carry = 0;
-    for (int i0 = 0; i0 <= p.ns; i0 += kPlanThreads) {
+    for (int i0 = 0; i0 <= p.ns; i0 += nt) {
         const int i = i0 + tid;
-        int v = p.ns > 0 && i <= p.ns ? min(max(p.starts[i], 0), p.rows) : 0;
-        int all;
-        v = block_incl_scan(v, shi, [](int a, int b) { return max(a, b); }, &all);
-        if (i <= p.ns) p.gs[i] = max(carry, v);
-        carry = max(carry, all);
+        int v[1] = {p.ns > 0 && i <= p.ns ? min(max(p.starts[i], 0), p.rows) : 0};
+        int all[1];
+        block_incl_scan<1>(v, shi, [](int a, int b) { return max(a, b); }, all);
+        if (i <= p.ns) {
+            p.gs[i] = max(carry, v[0]);
+            if (CACHED) s_gs[i] = max(carry, v[0]);
+        }
+        carry = max(carry, all[0]);
     }
     __syncthreads();
-    long long done = 0;
-    for (int i0 = 0; i0 < p.nsets; i0 += kPlanThreads) {
+    const int* gs = CACHED ? s_gs : p.gs;
+    long long done[2] = {0, 0};  // units, tiles
+    for (int i0 = 0; i0 < p.nsets; i0 += nt) {
         const int i = i0 + tid;
+        if (i0) lengths(i);
         SetDesc d = {};
-        long long amount = 0;
+        long long amount[2] = {0, 0};
         if (i < p.nsets) {
             if (i < p.ns) {
-                d.row0 = p.gs[i];
-                d.ntok = p.gs[i + 1] - d.row0;
-                const int n = max(p.set_lens[i], 0);
+                d.row0 = gs[i];
+                d.ntok = gs[i + 1] - d.row0;
+                const int n = max(len, 0);
                 if (p.paged) {
                     d.src = d.row0;
                     // a group of one row has nothing to share: all its keys are the row's own
                     d.khi = d.ntok > 1 ? min(n, p.max_keys) : 0;
                 } else {
-                    const long long end = min((long long)p.key_starts[i] + n, (long long)p.num_keys);
-                    d.src = max(p.key_starts[i], 0);
+                    const long long end = min((long long)key0 + n, (long long)p.num_keys);
+                    d.src = max(key0, 0);
                     d.khi = (int)max(end - d.src, 0ll);
                 }
             } else {
                 d.row0 = d.src = i - p.ns;
-                d.ntok = d.own = 1;
-                d.khi = min(p.seq_lens[d.row0], p.max_keys);
+                d.ntok = 1;
+                d.khi = min(len, p.max_keys);
                 int lo = 0, hi = p.ns + 1;  // starts that are <= row
                 while (lo < hi) {
                     const int mid = (lo + hi) >> 1;
-                    if (p.gs[mid] <= d.row0) lo = mid + 1;
+                    if (gs[mid] <= d.row0) lo = mid + 1;
                     else hi = mid;
                 }
-                if (lo >= 1 && lo <= p.ns && p.gs[lo] - p.gs[lo - 1] > 1) d.klo = max(p.set_lens[lo - 1], 0);
+                const bool in = lo >= 1 && lo <= p.ns && gs[lo] - gs[lo - 1] > 1;
+                if (in) d.klo = max(p.set_lens[lo - 1], 0);
+                d.own = in ? lo + 1 : 1;  // 2 + its group
             }
-            d.nb = (int)(((long long)d.ntok * p.G + p.RB - 1) / p.RB);
-            d.tiles = d.khi > d.klo ? (int)(((long long)d.khi - (d.klo & ~15) + 63) / 64) : 0;
-            amount = (long long)p.Hkv * d.nb * (p.whole ? 1 : d.tiles);
+            d.nb = (int)div_small((long long)d.ntok * p.G + p.RB - 1, p.RB);
+            d.tiles = d.ntok > 0 && d.khi > d.klo ? (int)(((long long)d.khi - (d.klo & ~15) + 63) / 64) : 0;
+            const long long items = (long long)p.Hkv * d.nb;
+            amount[0] = p.whole ? items : d.tiles ? items * (d.tiles + kItemCost) : 0;
+            amount[1] = items * d.tiles;
             p.desc[i] = d;
+            if (CACHED) s_desc[i] = d;
         }
-        long long all;
-        const long long incl = block_incl_scan(amount, shl, [](long long a, long long b) { return a + b; }, &all);
-        if (i < p.nsets) p.cum[i] = done + incl - amount;
-        done += all;
+        long long incl[2] = {amount[0], amount[1]}, all[2];
+        block_incl_scan<2>(incl, shl, [](long long a, long long b) { return a + b; }, all);
+        if (i < p.nsets) {
+            const long long u = done[0] + incl[0] - amount[0], v = done[1] + incl[1] - amount[1];
+            p.cum[i] = u;
+            if (CACHED) {
+                s_cum[i] = u;
+                s_cumt[i] = v;
+            } else {
+                p.cumt[i] = v;
+            }
+        }
+        done[0] += all[0];
+        done[1] += all[1];
     }
-    if (tid == 0) p.cum[p.nsets] = done;
+    if (tid == 0) p.cum[p.nsets] = done[0];
+    if (p.whole) return;
+    __syncthreads();
+    const long long* cum = CACHED ? s_cum : reinterpret_cast<const long long*>(p.cum);
+    const long long* cumt = CACHED ? s_cumt : reinterpret_cast<const long long*>(p.cumt);
+    const SetDesc* desc = CACHED ? s_desc : p.desc;
+    const long long total = done[0];
+    const int n = plan_ranges(total, p.grid, p.umin);
+    auto set_of = [&](long long u) {  // last set with cum <= u
+        int lo = 0, hi = p.nsets;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (cum[mid] <= u) lo = mid;
+            else hi = mid;
+        }
+        return lo;
+    };
+    for (int w = tid; w < p.grid; w += nt) {
+        RangeRec r = {};
+        if (w < n) {
+            const long long u0 = div_small((long long)w * total, n), u1 = div_small((long long)(w + 1) * total, n);
+            r.set = set_of(u0);
+            r.d = desc[r.set];
+            const int64_t t0 = tiles_before(r.d, cum[r.set], cumt[r.set], u0, &r);
+            int64_t t1 = done[1];
+            if (u1 < total) {
+                const int s1 = set_of(u1);
+                t1 = tiles_before(desc[s1], cum[s1], cumt[s1], u1, nullptr);
+            }
+            r.ntiles = (int)(t1 - t0);
+        }
+        p.range[w] = r;
+    }
+    if (!p.paged) return;
+    for (int b = tid; b < p.rows; b += nt) {
+        RowRec r = {};
+        const SetDesc own = desc[p.ns + b];
+        r.own_u = cum[p.ns + b];
+        r.own_tiles = own.tiles;
+        if (own.own > 1) {
+            const int j = own.own - 2;
+            const SetDesc d = desc[j];
+            r.grp_u = cum[j];
+            r.grp_tiles = d.tiles;
+            r.grp_nb = d.nb;
+            r.grp_row0 = d.row0;
+            r.grp_ntok = d.ntok;
+        }
+        p.row[b] = r;
+    }
 }
 
-// One wave per query head of a row: the pieces' rows, weighted by their maxima.
-// Paged: pieces of the group's common keys and of the row's own; contiguous: of
-// an item that ranges cut (whole ones are written already).
-template <int D, bool BF>
-__global__ void __launch_bounds__(256) shared_merge_kernel(TileParams p, int RB, int per_wave) {
+// the pieces of a row: of ranges w0 .. w0 + cnt - 1, first partial row base (of range 0)
+struct Pieces {
+    int w0[2], cnt[2];
+    int64_t base[2];
+};
+
+// sum over pieces first, first + step, .. of np: o, l against the running maximum m
+template <int D, typename PieceAt>
+__device__ __forceinline__ void merge_pieces(int first, int step, int np, int lane, PieceAt piece, float& m, float& l,
+                                             float (&acc)[D / 64]) {
     constexpr int NPL = D / 64;
     typedef float vec __attribute__((ext_vector_type(NPL == 1 ? 2 : NPL)));
-    const int lane = threadIdx.x & 63;
-    const int64_t total = p.cum[p.nsets];
-    const int n = plan_ranges(total, p.grid, p.umin);
-    const int64_t first = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * per_wave;
-    for (int64_t row = first; row < min(first + per_wave, (int64_t)p.total_rows * p.Hq); ++row) {
-        const int b = __builtin_amdgcn_readfirstlane((int)(row / p.Hq)), hq = __builtin_amdgcn_readfirstlane((int)(row % p.Hq));
-        const int g = hq / p.G;
-        int w0[2] = {0, 0}, cnt[2] = {0, 0};  // first range and pieces: common keys, own keys
-        int64_t base[2] = {0, 0};             // partial row of range 0
-        auto set_pieces = [&](int k, int s) __attribute__((always_inline)) {
-            const SetDesc d = p.desc[s];
-            if (d.tiles == 0) return;
-            const int r = (b - d.row0) * p.G + hq % p.G, rb = r / RB;
-            const int64_t u = p.cum[s] + ((int64_t)g * d.nb + rb) * d.tiles;
-            w0[k] = plan_range_of(u, total, n);
-            cnt[k] = plan_range_of(u + d.tiles - 1, total, n) - w0[k] + 1;
-            base[k] = (p.paged ? plan_rows_paged(0, RB, p.Hq, p.G, p.total_rows, d, g, rb) : 0) + r % RB;
-        };
-        const int j = p.ns > 0 ? plan_find(p.gs, p.ns + 1, b, lane) : -1;
-        const bool in_set = p.ns > 0 && p.gs[0] <= b && j < p.ns;
-        if (in_set) set_pieces(0, j);
-        if (p.paged) set_pieces(1, p.ns + b);
-        else if (!in_set || cnt[0] == 1) continue;  // padding, or written
-        const int np = cnt[0] + cnt[1];
-        auto piece = [&](int i) __attribute__((always_inline)) -> const float* {
-            const int k = i >= cnt[0] ? 1 : 0, w = w0[k] + i - (k ? cnt[0] : 0);
-            const int64_t at = p.paged ? (int64_t)w * RB + base[k] : plan_rows_local(w, RB, i > 0) + base[0];
-            return p.part + at * (D + 4);
-        };
-        float mx = -__builtin_inff();
-        for (int i = lane; i < np; i += 64) mx = fmaxf(mx, piece(i)[D]);
+    m = -__builtin_inff();
+    l = 0.0f;
 #pragma unroll
-        for (int m = 32; m >= 1; m >>= 1) mx = fmaxf(mx, shfl_xor(mx, m));
-        float acc[NPL], l = 0.0f;
+    for (int e = 0; e < NPL; ++e) acc[e] = 0.0f;
+    constexpr int U = 8;
+    for (int i0 = first; i0 < np; i0 += U * step) {
+        float x[U][NPL];
+        float2 ml[U];
 #pragma unroll
-        for (int e = 0; e < NPL; ++e) acc[e] = 0.0f;
-        for (int i0 = 0; i0 < np; i0 += 64) {
-            float wt = 0.0f;
-            if (i0 + lane < np) {
-                const float2 ml = *reinterpret_cast<const float2*>(piece(i0 + lane) + D);
-                wt = ml.x == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(ml.x - mx);
-                l += wt == 0.0f ? 0.0f : wt * ml.y;
-            }
-            const int m = min(64, np - i0);
-#pragma unroll 8
-            for (int i = 0; i < m; ++i) {
-                const float wi = shfl(wt, i);
-                const float* s = piece(i0 + i) + NPL * lane;
-                float x[NPL];
-                if constexpr (NPL == 1) x[0] = s[0];
-                else {
-                    const vec y = *reinterpret_cast<const vec*>(s);
+        for (int i = 0; i < U; ++i) {
+            const float* s = piece(min(i0 + i * step, np - 1));
+            ml[i] = *reinterpret_cast<const float2*>(s + D);
+            if constexpr (NPL == 1) x[i][0] = s[lane];
+            else {
+                const vec y = *reinterpret_cast<const vec*>(s + NPL * lane);
 #pragma unroll
-                    for (int e = 0; e < NPL; ++e) x[e] = y[e];
-                }
-                // a piece of weight 0 adds nothing, not 0 * inf
-#pragma unroll
-                for (int e = 0; e < NPL; ++e) acc[e] = wi == 0.0f ? acc[e] : __builtin_fmaf(wi, x[e], acc[e]);
+                for (int e = 0; e < NPL; ++e) x[i][e] = y[e];
             }
         }
+        float mx = m;
 #pragma unroll
-        for (int m = 32; m >= 1; m >>= 1) l += shfl_xor(l, m);
+        for (int i = 0; i < U; ++i) mx = fmaxf(mx, i0 + i * step < np ? ml[i].x : -__builtin_inff());
+        const float a = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - mx);
+        m = mx;
+        l = a == 0.0f ? 0.0f : l * a;
+#pragma unroll
+        for (int e = 0; e < NPL; ++e) acc[e] = a == 0.0f ? 0.0f : acc[e] * a;
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            // (a piece of weight 0 adds nothing, not 0 * inf; a NaN reference stays one)
+            const bool in = i0 + i * step < np && ml[i].x != -__builtin_inff();
+            const float wt = in ? __builtin_amdgcn_exp2f(ml[i].x - mx) : 0.0f;
+            l = wt == 0.0f ? l : __builtin_fmaf(wt, ml[i].y, l);
+#pragma unroll
+            for (int e = 0; e < NPL; ++e) acc[e] = wt == 0.0f ? acc[e] : __builtin_fmaf(wt, x[i][e], acc[e]);
+        }
+    }
+}
+
+// Paged calls: one workgroup per row and query head; its waves take every fourth piece
+// of the group's common keys and of the row's own.
+template <int D, bool BF>
+__global__ void __launch_bounds__(256) shared_merge_paged_kernel(TileParams p, int RB) {
+    constexpr int NPL = D / 64;
+    __shared__ float so[4][D], sml[4][2];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int b = blockIdx.x / p.Hq, hq = blockIdx.x % p.Hq, g = hq / p.G;
+    const int64_t total = p.cum[p.nsets];
+    const RowRec rec = p.row[b];
+    const int n = plan_ranges(total, p.grid, p.umin);
+    Pieces pc = {};
+    if (rec.grp_tiles) {
+        const int r = (b - rec.grp_row0) * p.G + hq % p.G, rb = r / RB;
+        const int64_t u = rec.grp_u + ((int64_t)g * rec.grp_nb + rb) * (rec.grp_tiles + kItemCost) + kItemCost;
+        pc.w0[0] = plan_range_of(u, total, n);
+        pc.cnt[0] = plan_range_of(u + rec.grp_tiles - 1, total, n) - pc.w0[0] + 1;
+        pc.base[0] = plan_rows_paged(0, RB, p.Hq, p.G, p.total_rows, 0, rec.grp_row0, rec.grp_ntok, g, rb) + r % RB;
+    }
+    if (rec.own_tiles) {
+        const int r = hq % p.G, rb = r / RB, nb = (p.G + RB - 1) / RB;
+        const int64_t u = rec.own_u + ((int64_t)g * nb + rb) * (rec.own_tiles + kItemCost) + kItemCost;
+        pc.w0[1] = plan_range_of(u, total, n);
+        pc.cnt[1] = plan_range_of(u + rec.own_tiles - 1, total, n) - pc.w0[1] + 1;
+        pc.base[1] = plan_rows_paged(0, RB, p.Hq, p.G, p.total_rows, 1, b, 1, g, rb) + r % RB;
+    }
+    auto piece = [&](int i) __attribute__((always_inline)) -> const float* {
+        const int k = i >= pc.cnt[0] ? 1 : 0;
+        const int at = (k ? pc.w0[1] - pc.cnt[0] : pc.w0[0]) + i;
+        return p.part + ((int64_t)at * RB + (k ? pc.base[1] : pc.base[0])) * (D + 4);
+    };
+    float m, l, acc[NPL];
+    merge_pieces<D>(w, 4, pc.cnt[0] + pc.cnt[1], lane, piece, m, l, acc);
+#pragma unroll
+    for (int e = 0; e < NPL; ++e) so[w][NPL * lane + e] = acc[e];
+    if (lane == 0) {
+        sml[w][0] = m;
+        sml[w][1] = l;
+    }
+    __syncthreads();
+    if (threadIdx.x >= D) return;
+    float mx = sml[0][0];
+#pragma unroll
+    for (int i = 1; i < 4; ++i) mx = fmaxf(mx, sml[i][0]);
+    float o = 0.0f, ls = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float wt = sml[i][0] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(sml[i][0] - mx);
+        o = wt == 0.0f ? o : __builtin_fmaf(wt, so[i][threadIdx.x], o);
+        ls = wt == 0.0f ? ls : __builtin_fmaf(wt, sml[i][1], ls);
+    }
+    p.out[(int64_t)blockIdx.x * D + threadIdx.x] = f32_to_half<BF>(ls == 0.0f ? 0.0f : o / ls);
+}
+
+// Contiguous calls: workgroup (x, y) has the item that range x begins and does not
+// finish, if there is one (whole items are written already), and 16 of its
+// rows; and sets without keys, whose rows are zero.
+template <int D, bool BF>
+__global__ void __launch_bounds__(256) shared_merge_local_kernel(TileParams p, int RB) {
+    constexpr int NPL = D / 64;
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int w = blockIdx.x;
+    for (int s = w; s < p.ns; s += p.grid) {
+        const SetDesc d = p.desc[s];
+        if (d.tiles) continue;
+        const int64_t n = (int64_t)d.ntok * p.Hq * D / 8;
+        for (int64_t i = (int64_t)blockIdx.y * 256 + threadIdx.x; i < n; i += 256 * (int64_t)gridDim.y)
+            *reinterpret_cast<u32x4*>(p.out + (int64_t)d.row0 * p.Hq * D + 8 * i) = u32x4{0u, 0u, 0u, 0u};
+    }
+    if (w + 1 >= p.grid) return;
+    const RangeRec rec = p.range[w + 1], me = p.range[w];
+    // the next range begins inside an item, which began here: not before this range
+    if (rec.t == 0 || (me.set == rec.set && me.g == rec.g && me.rb == rec.rb && me.t > 0)) return;
+    const int nrow = min(RB, rec.d.ntok * p.G - RB * rec.rb), r0 = 16 * blockIdx.y + 4 * wv;
+    if (r0 >= nrow) return;
+    const int64_t total = p.cum[p.nsets];
+    const int n = plan_ranges(total, p.grid, p.umin);
+    const int64_t last = p.cum[rec.set] + ((int64_t)rec.g * rec.d.nb + rec.rb + 1) * (rec.d.tiles + kItemCost) - 1;
+    const int cnt = plan_range_of(last, total, n) - w + 1;
+    for (int r = r0; r < min(r0 + 4, nrow); ++r) {
+        auto piece = [&](int i) __attribute__((always_inline)) -> const float* {
+            return p.part + (plan_rows_local(w + i, RB, i > 0) + r) * (D + 4);
+        };
+        float m, l, acc[NPL];
+        merge_pieces<D>(0, 1, cnt, lane, piece, m, l, acc);
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        uint16_t* op = p.out + row * D + NPL * lane;
+        const int x = RB * rec.rb + r;
+        uint16_t* op = p.out + ((rec.d.row0 + x / p.G) * (int64_t)p.Hq + rec.g * p.G + x % p.G) * D + NPL * lane;
 #pragma unroll
         for (int e = 0; e < NPL; ++e) op[e] = f32_to_half<BF>(acc[e] * inv);
     }
 }
 
+template <int D, bool BF>
+void launch_merge_d(const TileParams& p, int RB, hipStream_t s) {
+    if (p.paged) {
+        const int64_t rows = (int64_t)p.total_rows * p.Hq;
+        hipLaunchKernelGGL((shared_merge_paged_kernel<D, BF>), dim3((unsigned)rows), dim3(256), 0, s, p, RB);
+        return;
+    }
+    hipLaunchKernelGGL((shared_merge_local_kernel<D, BF>), dim3((unsigned)p.grid, (unsigned)RB / 16), dim3(256), 0, s, p,
+                       RB);
+}
+
 int launch_merge(const TileParams& p, int D, bool bf, int RB, hipStream_t s) {
-    // a wave takes several rows where they are more than fill the chip
-    const int64_t rows = (int64_t)p.total_rows * p.Hq;
-    const int per = (int)((rows + 32767) / 32768);
-    const dim3 grid((unsigned)((rows + 4 * per - 1) / (4 * per))), block(256);
-    if (D == 64 && bf) hipLaunchKernelGGL((shared_merge_kernel<64, true>), grid, block, 0, s, p, RB, per);
-    else if (D == 64) hipLaunchKernelGGL((shared_merge_kernel<64, false>), grid, block, 0, s, p, RB, per);
-    else if (D == 128 && bf) hipLaunchKernelGGL((shared_merge_kernel<128, true>), grid, block, 0, s, p, RB, per);
-    else if (D == 128) hipLaunchKernelGGL((shared_merge_kernel<128, false>), grid, block, 0, s, p, RB, per);
-    else if (bf) hipLaunchKernelGGL((shared_merge_kernel<256, true>), grid, block, 0, s, p, RB, per);
-    else hipLaunchKernelGGL((shared_merge_kernel<256, false>), grid, block, 0, s, p, RB, per);
+    switch (D) {
+        case 64: bf ? launch_merge_d<64, true>(p, RB, s) : launch_merge_d<64, false>(p, RB, s); break;
+        case 128: bf ? launch_merge_d<128, true>(p, RB, s) : launch_merge_d<128, false>(p, RB, s); break;
+        default: bf ? launch_merge_d<256, true>(p, RB, s) : launch_merge_d<256, false>(p, RB, s); break;
+    }
     VMC_LAUNCH_CHECK();
     return VMC_OK;
 }
 
 // How a call runs, from its sizes alone (lengths are on the device).
 struct Shape {
-    int waves, whole, grid;  // waves of a workgroup; one item each; ranges (whole: workgroups)
-    size_t cum, desc, gs, part, bytes;  // workspace offsets, size
+    int whole, grid;  // one item a workgroup; ranges (whole: workgroups)
+    bool conv;        // bf16 V is converted to fp16
+    size_t cum, cumt, desc, range, row, gs, part, bytes;  // workspace offsets, size
 };
 
 Shape shape_of(bool paged, int rows, int nsets, int Hq, int Hkv, int D) {
     Shape sh = {};
-    const int64_t G = Hq / Hkv;
+    const int64_t G = Hq / Hkv, sets = std::max(nsets, 1);
     // workgroups that fit a CU: 64 KB of tiles each (head_dim 256: 128 KB)
-    const int per_cu = D == 256 ? 1 : 2;
-    sh.waves = 4;
-    const int64_t items = (int64_t)Hkv * ((rows * G) / 256 + std::min(rows, nsets));
-    // whole items of 256 rows where they are many times the CUs
-    if (!paged && rows * G >= (int64_t)128 * nsets && items >= 4 * (int64_t)num_cus() && items < (1 << 30)) {
-        sh.waves = 8;
+    sh.grid = num_cus() * (D == 256 ? 1 : 2);
+    // Whole items where sets of many rows give several times the workgroups
+    const int64_t items = (int64_t)Hkv * (rows * G / kTileRows + std::min<int64_t>(rows, sets));
+    if (!paged && rows * G >= kTileRows * sets && items >= 4 * (int64_t)sh.grid && items < (1 << 30)) {
         sh.whole = 1;
         sh.grid = (int)((items + 7) & ~7);
-    } else {
-        sh.grid = num_cus() * per_cu;
     }
+    sh.conv = rows * G >= 64 * sets;
     const int64_t total = paged ? (int64_t)nsets + rows : nsets;
-    const int64_t RB = 32 * sh.waves;
-    const int64_t prow = sh.whole ? 0 : paged ? sh.grid * RB + 2 * (int64_t)rows * Hq : 2 * sh.grid * RB;
+    const int64_t prow = sh.whole ? 0 : paged ? (int64_t)sh.grid * kTileRows + 2 * (int64_t)rows * Hq : 2 * (int64_t)sh.grid * kTileRows;
     auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
     sh.cum = 0;
-    sh.desc = up((size_t)(total + 1) * sizeof(int64_t));
-    sh.gs = sh.desc + up((size_t)total * sizeof(SetDesc));
+    sh.cumt = up((size_t)(total + 1) * sizeof(int64_t));
+    sh.desc = 2 * sh.cumt;
+    sh.range = sh.desc + up((size_t)total * sizeof(SetDesc));
+    sh.row = sh.range + (sh.whole ? 0 : up((size_t)sh.grid * sizeof(RangeRec)));
+    sh.gs = sh.row + (paged ? up((size_t)rows * sizeof(RowRec)) : 0);
     sh.part = sh.gs + up((size_t)(nsets + 1) * sizeof(int32_t));
     sh.bytes = sh.part + (size_t)prow * (D + 4) * sizeof(float);
     return sh;
@@ -254,13 +440,20 @@ int shared_tiles(const SharedArgs& a, void* ws, hipStream_t s) {
     pl.num_keys = a.num_keys;
     pl.Hkv = a.Hkv;
     pl.G = a.Hq / a.Hkv;
-    pl.RB = 32 * sh.waves;
+    pl.RB = kTileRows;
     pl.paged = paged;
     pl.whole = sh.whole;
     pl.cum = reinterpret_cast<int64_t*>(w + sh.cum);
+    pl.cumt = reinterpret_cast<int64_t*>(w + sh.cumt);
     pl.desc = reinterpret_cast<SetDesc*>(w + sh.desc);
+    pl.range = reinterpret_cast<RangeRec*>(w + sh.range);
+    pl.row = reinterpret_cast<RowRec*>(w + sh.row);
+    pl.grid = sh.grid;
+    pl.umin = kUnitsMin;
     pl.gs = reinterpret_cast<int32_t*>(w + sh.gs);
-    hipLaunchKernelGGL(shared_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, pl);
+    const int threads = pl.nsets > 512 || sh.grid > 512 ? kPlanThreads : 512;
+    if (pl.nsets <= kPlanCached) hipLaunchKernelGGL(shared_plan_kernel<true>, dim3(1), dim3(threads), 0, s, pl);
+    else hipLaunchKernelGGL(shared_plan_kernel<false>, dim3(1), dim3(threads), 0, s, pl);
     VMC_LAUNCH_CHECK();
 
     TileParams p = {};
@@ -274,6 +467,8 @@ int shared_tiles(const SharedArgs& a, void* ws, hipStream_t s) {
     p.scale = a.scale;
     p.cum = pl.cum;
     p.desc = pl.desc;
+    p.range = pl.range;
+    p.row = pl.row;
     p.gs = pl.gs;
     p.ns = a.nsets;
     p.nsets = pl.nsets;
@@ -281,7 +476,7 @@ int shared_tiles(const SharedArgs& a, void* ws, hipStream_t s) {
     p.whole = sh.whole;
     p.total_rows = a.rows;
     p.grid = sh.grid;
-    p.umin = 2;
+    p.umin = kUnitsMin;
     p.part = reinterpret_cast<float*>(w + sh.part);
     if (paged) {
         p.kp = a.kp;
@@ -303,9 +498,9 @@ int shared_tiles(const SharedArgs& a, void* ws, hipStream_t s) {
     }
     const int src = !paged ? 0 : a.src == GEN_Q8 ? 2 : a.src == GEN_Q4 ? 3 : 1;
     const bool bf = a.q_bf16 != 0;
-    const int rc = a.D == 64    ? shared_tile_d64(p, src, bf, sh.waves, sh.grid, s)
-                   : a.D == 128 ? shared_tile_d128(p, src, bf, sh.waves, sh.grid, s)
-                                : shared_tile_d256(p, src, bf, sh.waves, sh.grid, s);
+    const int rc = a.D == 64    ? shared_tile_d64(p, src, bf, sh.conv, sh.grid, s)
+                   : a.D == 128 ? shared_tile_d128(p, src, bf, sh.conv, sh.grid, s)
+                                : shared_tile_d256(p, src, bf, sh.conv, sh.grid, s);
     if (rc != VMC_OK || sh.whole) return rc;
     return launch_merge(p, a.D, bf, pl.RB, s);
 }

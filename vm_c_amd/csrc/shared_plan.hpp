@@ -22,6 +22,29 @@ struct SetDesc {
     int own;         // paged: a row's own keys (else each row has seq_lens[row] at most)
 };
 
+// Where a range begins: its first tile, and how many it has.
+struct RangeRec {
+    int set, g, rb, t, ntiles;
+    int pad[3];
+    SetDesc d;  // of the set
+};
+
+// Paged calls: what the merge needs of one row.
+struct RowRec {
+    int64_t own_u, grp_u;       // first unit of the set's first item
+    int own_tiles;              // 0: none
+    int grp_tiles, grp_nb, grp_row0, grp_ntok;
+    int pad[3];
+};
+
+// An item's first kItemCost units stand for what a workgroup spends on the item beside
+// its tiles (the next rows' Q, the last rows' partial results), so that a range of
+// short items gets fewer tiles.
+constexpr int kItemCost = 2;
+
+constexpr int kTileWaves = 4;  // waves of the shared-keys kernel, 32 rows each
+constexpr int kTileRows = 32 * kTileWaves;  // rows of an item
+
 struct PlanParams {
     const int32_t* starts;
     const int32_t* set_lens;
@@ -32,9 +55,13 @@ struct PlanParams {
     int max_keys, num_keys;
     int Hkv, G, RB;
     int paged, whole;
-    int64_t* cum;   // [nsets + 1] units (whole: items) before each set
-    SetDesc* desc;  // [nsets]
-    int32_t* gs;    // [ns + 1] starts, cut to [0, rows] and made non-decreasing
+    int grid, umin;   // ranges, and the fewest units of one
+    int64_t* cum;     // [nsets + 1] units (whole: items) before each set
+    int64_t* cumt;    // [nsets + 1] tiles before each set
+    SetDesc* desc;    // [nsets]
+    RangeRec* range;  // [grid] (not whole)
+    RowRec* row;      // [rows] (paged)
+    int32_t* gs;      // [ns + 1] starts, cut to [0, rows] and made non-decreasing
 };
 
 struct TileParams {
@@ -45,6 +72,8 @@ struct TileParams {
     float scale;
     const int64_t* cum;
     const SetDesc* desc;
+    const RangeRec* range;
+    const RowRec* row;
     const int32_t* gs;
     int ns, nsets, paged, whole;
     int total_rows;
@@ -59,9 +88,9 @@ struct TileParams {
     const int32_t* seq_lens;
 };
 
-int shared_tile_d64(const TileParams& p, int src, bool q_bf16, int waves, unsigned grid, hipStream_t s);
-int shared_tile_d128(const TileParams& p, int src, bool q_bf16, int waves, unsigned grid, hipStream_t s);
-int shared_tile_d256(const TileParams& p, int src, bool q_bf16, int waves, unsigned grid, hipStream_t s);
+int shared_tile_d64(const TileParams& p, int src, bool q_bf16, bool conv, unsigned grid, hipStream_t s);
+int shared_tile_d128(const TileParams& p, int src, bool q_bf16, bool conv, unsigned grid, hipStream_t s);
+int shared_tile_d256(const TileParams& p, int src, bool q_bf16, bool conv, unsigned grid, hipStream_t s);
 
 // The MFMA path of a call: whether it takes the shape, what workspace it needs (its
 // sizes alone decide), and the launches.
@@ -79,7 +108,9 @@ __host__ __device__ __forceinline__ int plan_ranges(int64_t total, int grid, int
 
 // the range that holds unit u of total, ranges w being [w total / n, (w + 1) total / n)
 __device__ __forceinline__ int plan_range_of(int64_t u, int64_t total, int n) {
-    return (int)(((u + 1) * n - 1) / total);
+    const int64_t x = (u + 1) * n - 1;
+    if (((x | total) >> 32) == 0) return (int)((uint32_t)x / (uint32_t)total);
+    return (int)(x / total);
 }
 
 // last s in [0, n) with cum[s] <= u (cum non-decreasing, cum[0] <= u); one wave, 64
@@ -102,9 +133,9 @@ __device__ __forceinline__ int plan_find(const T* cum, int n, int64_t u, int lan
 // the axis, where each step goes to the next item or the next range: range *
 // rb_rows + (rows of the items before) grows by at least a piece's rows with
 // each step.  grid * rb_rows + 2 * rows * Hq rows in all.
-__device__ __forceinline__ int64_t plan_rows_paged(int range, int rb_rows, int Hq, int G, int rows, const SetDesc& d,
-                                                   int g, int rb) {
-    return (int64_t)range * rb_rows + (int64_t)Hq * ((d.own ? rows : 0) + (int64_t)d.row0) + (int64_t)g * d.ntok * G +
+__device__ __forceinline__ int64_t plan_rows_paged(int range, int rb_rows, int Hq, int G, int rows, int own, int row0,
+                                                   int ntok, int g, int rb) {
+    return (int64_t)range * rb_rows + (int64_t)Hq * ((own ? rows : 0) + (int64_t)row0) + (int64_t)g * ntok * G +
            rb * rb_rows;
 }
 

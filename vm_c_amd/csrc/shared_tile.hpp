@@ -25,9 +25,17 @@
 // blocks through registers, dequantized to fp16 (code * d rounded once: 2^-11
 // of a value at most).
 //
-// Weights enter P . V as two 16-bit terms of V's type, which leave 2^-17 (bf16)
-// or 2^-23 (fp16) of a weight; one term would double the rounding error of the
-// 16-bit result (its 2^-9 and the weights' 2^-9 in bf16).
+// Weights enter P . V as fp16 where that costs nothing the result shows: half a step is
+// 2^-11 of a weight, beside the 2^-8 of a bf16 result.  bf16 V becomes fp16 for
+// it, by the waves that fetched its rows, while slower waves still multiply:
+// each 16 keys times 2^8 (values up to 255), 1 (larger ones) or 2^20 (all below
+// 2^-12), which their weights undo against the largest of an item's.  So values from
+// 2^-33 to 65504 keep their bits; the smaller ones of a chunk are off by 2^-25 over
+// its scale at most.  A chunk outside that range
+// makes its rows rerun.  Elsewhere (fp16 results; few rows, where the products
+// are not what counts) weights are two 16-bit terms of V's type, which leave
+// 2^-17 (bf16) or 2^-23 (fp16) of a weight: one term of 8 bits, or of the result's
+// own 11, would add as much error as the rounding of the result.
 #pragma once
 
 #include "generic_row.hpp"
@@ -116,24 +124,30 @@ __device__ __noinline__ void shared_row_exact(const uint16_t* q, const uint8_t* 
 
 // BF: the products' type (LOCAL and PAGED: the rows'; GGUF: fp16, BF false);
 // QBF: the type of q and out
-template <int D, int SRC, bool QBF, int W>
-__global__ void __launch_bounds__(64 * W, 2) shared_tile_kernel(TileParams p) {
+template <int D, int SRC, bool QBF, bool CONV>
+__global__ void __launch_bounds__(256, D == 256 ? 1 : 2) shared_tile_kernel(TileParams p) {
+    constexpr int W = kTileWaves;
     constexpr bool kGguf = SRC == TS_Q8 || SRC == TS_Q4;
     constexpr bool BF = QBF && !kGguf;
     using M = MT<BF>;
     using V8 = typename M::v8;
     constexpr int ROW = 2 * D, TILE = kBN * ROW;
-    constexpr int NS = kGguf || D == 256 || (D == 128 && W == 4) ? 2 : 3;  // tile slots
-    constexpr int NTR = TILE / (1024 * W);    // transfers per wave and tensor
-    constexpr int HB = D == 256 ? 1 : 2;      // 32-key blocks per softmax round
-    constexpr float kOff = BF ? 0.0f : 7.0f;  // weights are 2^(s - m + kOff), at most 2^15
-    constexpr int RB = 32 * W;                // rows of an item
+    constexpr int NS = kGguf || D != 64 ? 2 : 3;      // slots
+    constexpr int NTR = TILE / (1024 * W);            // transfers per wave and tensor
+    constexpr int RB = 32 * W;                        // rows of an item
+    constexpr bool kConv = CONV;                      // bf16 V is converted to fp16
+    static_assert(!CONV || BF, "fp16 V needs no conversion");
+    constexpr bool PBF = BF && !kConv;                // the type of P . V
+    constexpr int NT = PBF || !QBF ? 2 : 1;           // terms of a weight
+    constexpr float kOff = PBF ? 0.0f : 7.0f;         // weights are 2^(s - m + kOff), at most 2^15
+    constexpr int HB = D == 256 ? 1 : 2;              // 32-key blocks per softmax round
     // GGUF: blocks per lane and tile (K's then V's), dwords from a block's 4-byte floor
     constexpr int NBL = D / (16 * W) > 0 ? D / (16 * W) : 1;
     constexpr int BE = SRC == TS_Q8 ? 34 : 18, NWD = SRC == TS_Q8 ? 9 : 5;
     struct Lds {
-        uint8_t tile[NS][2][TILE];  // [slot][K, V]
-        float qs[W][D];             // rows that rerun key by key
+        uint8_t tile[NS][2][TILE];                       // [slot][K, V]
+        float qs[W][D];                                  // rows that rerun key by key
+        alignas(16) float vexp[2][W];                    // kConv [tile][16-key chunk]: 8 - log2 of V's scale
     };
     __shared__ __attribute__((aligned(1024))) Lds lds;
 
@@ -141,159 +155,192 @@ __global__ void __launch_bounds__(64 * W, 2) shared_tile_kernel(TileParams p) {
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int c32 = lane & 31, h = lane >> 5;
 
-    // ---- this workgroup's range of the axis
-    int range;
-    int64_t u0, u1;
-    const int64_t total = as_const(p.cum)[p.nsets];
-    if (p.whole) {  // one item; consecutive items to one XCD, whose L2 holds their keys
-        const int64_t per = (total + 7) >> 3;
-        range = (int)((blockIdx.x & 7) * per + (blockIdx.x >> 3));
-        if ((blockIdx.x >> 3) >= per || range >= total) return;
-        u0 = range;
-        u1 = range + 1;
-    } else {
-        const int n = plan_ranges(total, p.grid, p.umin);
-        range = n == p.grid && (n & 7) == 0 ? (int)((blockIdx.x & 7) * (n >> 3) + (blockIdx.x >> 3)) : (int)blockIdx.x;
-        if (range >= n) return;
-        u0 = range * total / n;
-        u1 = (range + 1) * total / n;
-        if (u0 >= u1) return;
-    }
-    struct Cursor {
-        int set, g, rb, t;
-        SetDesc d;
+    // The parameters as rare steps read them: from the kernel's arguments in memory, there
+    // and then, as the compiler would otherwise keep each in scalar registers from
+    // the start and spill those (to vector lanes, read back in every tile)
+    auto arg = [&]() __attribute__((always_inline)) {
+        auto a = (const __attribute__((address_space(4))) TileParams*)__builtin_amdgcn_kernarg_segment_ptr();
+        asm volatile("" : "+s"(a));
+        return a;
     };
-    auto load_desc = [&](Cursor& c) __attribute__((always_inline)) {
-        const auto* s = as_const(reinterpret_cast<const int*>(p.desc + c.set));
-        c.d = SetDesc{s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7]};
+    // ---- this workgroup's tiles.  Of a set, a cursor keeps what each tile needs; the rest
+    // is read again (through the scalar cache) where an item begins or ends.
+    struct Cursor {
+        int set, g, rb, t, tiles, nb, klo, khi, src;
+    };
+    auto desc_of = [&](int set) __attribute__((always_inline)) {
+        const auto* s = as_const(reinterpret_cast<const int*>(arg()->desc + set));
+        return SetDesc{s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7]};
+    };
+    auto take = [&](Cursor& c, const SetDesc& d) __attribute__((always_inline)) {
+        c.tiles = d.tiles;
+        c.nb = d.nb;
+        c.klo = d.klo;
+        c.khi = d.khi;
+        c.src = d.src;
     };
     auto advance = [&](Cursor& c) __attribute__((always_inline)) {
-        if (++c.t < c.d.tiles) return;
+        if (++c.t < c.tiles) return;
         c.t = 0;
-        if (++c.rb < c.d.nb) return;
+        if (++c.rb < c.nb) return;
         c.rb = 0;
-        if (++c.g < p.Hkv) return;
+        if (++c.g < arg()->Hkv) return;
         c.g = 0;
         do {
-            if (++c.set >= p.nsets) return;  // past the axis: not used
-            load_desc(c);
-        } while (c.d.tiles == 0);
+            if (++c.set >= arg()->nsets) return;  // past the axis: not used
+            take(c, desc_of(c.set));
+        } while (c.tiles == 0);
     };
-    Cursor cc;
-    cc.set = plan_find(p.cum, p.nsets, u0, lane);
-    load_desc(cc);
-    {
-        const int64_t rem = u0 - as_const(p.cum)[cc.set];
-        const int per = p.whole ? 1 : cc.d.tiles;
-        const int item = (int)(rem / per);
-        cc.t = (int)(rem % per);
-        cc.g = item / cc.d.nb;
-        cc.rb = item % cc.d.nb;
+    Cursor cc;  // of the tile in use
+    int range = blockIdx.x, units;
+    if (arg()->whole) {  // one item; consecutive items to one XCD, whose L2 holds their keys
+        const int64_t total = as_const(p.cum)[p.nsets], per = (total + 7) >> 3;
+        const int64_t item = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+        if ((blockIdx.x >> 3) >= per || item >= total) return;
+        cc.set = plan_find(p.cum, p.nsets, item, lane);
+        take(cc, desc_of(cc.set));
+        const int in_set = (int)(item - as_const(p.cum)[cc.set]);
+        cc.t = 0;
+        cc.g = in_set / cc.nb;
+        cc.rb = in_set % cc.nb;
+        units = cc.tiles;
+    } else {
+        const auto* r = as_const(reinterpret_cast<const int*>(p.range + range));
+        cc.set = r[0];
+        cc.g = r[1];
+        cc.rb = r[2];
+        cc.t = r[3];
+        units = r[4];
+        take(cc, SetDesc{r[8], r[9], r[10], r[11], r[12], r[13], r[14], r[15]});
+        if (units == 0) return;
     }
-    int units = p.whole ? cc.d.tiles : (int)(u1 - u0);  // to go
-    Cursor pc = cc;
+    units = __builtin_amdgcn_readfirstlane(units);
 
-    // ---- fetch side.  A record names the tile to load next: base addresses of
-    // this wave's rows (TS_LOCAL, TS_PAGED) or of the four pages
-    const uint8_t *rk[kGguf ? 4 : 1], *rv[kGguf ? 4 : 1];
-    int r_first = 0, r_last = 0;  // the wave's rows (GGUF: the tile's) clamp to these
-    uint32_t r_valid = 0, vq = 0;  // 16-key chunks that hold keys: the record's, and those of loaded tiles
-    auto fetch = [&]() __attribute__((always_inline)) {  // pc's tile
-        const int k0 = (pc.d.klo & ~15) + kBN * pc.t, last = pc.d.khi - 1 - k0;
-        const int first = max(pc.d.klo - k0, 0);
+    // ---- fetch side.  A record names a tile's memory: the offset of this wave's rows
+    // (TS_LOCAL, TS_PAGED) or of the four 16-key chunks (GGUF), and the rows that all
+    // others clamp to, so that each row read is a key of the item
+    constexpr int NA = kGguf ? 4 : 1;
+    struct Rec {
+        int64_t k[NA], v;  // (paged: k for both)
+        int first, last;
+    };
+    Cursor pc = cc;
+    Rec rec;            // of the next tile to load
+    uint32_t vq = 0;    // 16-key chunks that hold keys, 4 bits a tile, the latest fetched lowest
+    int fetched = 0;    // tiles with a record
+    auto fetch = [&]() __attribute__((always_inline)) {
+        if (fetched == units) return;
+        if (fetched) advance(pc);
+        ++fetched;
+        const int k0 = (pc.klo & ~15) + kBN * pc.t, last = pc.khi - 1 - k0;
+        rec.first = max(pc.klo - k0, 0);
+        rec.last = last;
         if constexpr (SRC == TS_LOCAL) {
-            const int64_t key = (int64_t)pc.d.src + k0;
-            rk[0] = p.kp + key * p.k_row + pc.g * p.k_head;
-            rv[0] = p.vp + key * p.v_row + pc.g * p.v_head;
-            r_first = first;
-            r_last = last;
-            r_valid = (2u << min(3, last >> 4)) - 1u;
+            const int64_t key = (int64_t)pc.src + k0;
+            rec.k[0] = key * p.k_row + pc.g * p.k_head;
+            rec.v = key * p.v_row + pc.g * p.v_head;
+            vq = (vq << 4) | ((2u << min(3, last >> 4)) - 1u);
         } else {
-            const auto* bt = as_const(p.bt + (int64_t)pc.d.src * p.max_blocks);
+            const auto* bt = as_const(p.bt + (int64_t)pc.src * p.max_blocks);
             int id[4];
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 const int k = k0 + 16 * min(c, last >> 4);
                 id[c] = bt[p.bs == 16 ? k >> 4 : k / p.bs];
             }
-            r_valid = 0;
-            int any = 0;  // a page for the rows of holes: their keys are masked, so it only has to be finite memory
+            uint32_t valid = 0;
+            int any = 0;  // a page for the rows of holes: their keys are masked
 #pragma unroll
             for (int c = 3; c >= 0; --c) {
-                r_valid |= id[c] >= 0 && 16 * c <= last ? 1u << c : 0u;
+                valid |= id[c] >= 0 && 16 * c <= last ? 1u << c : 0u;
                 any = id[c] >= 0 ? id[c] : any;
             }
-            r_first = first;
-            r_last = last;
-            auto at = [&](int c, int page, const uint8_t*& a, const uint8_t*& b) __attribute__((always_inline)) {
+            vq = (vq << 4) | valid;
+            auto at = [&](int c, int page) __attribute__((always_inline)) {
                 const int k = k0 + 16 * min(c, last >> 4);
                 const int in_page = p.bs == 16 ? 0 : k % p.bs;
-                const int64_t off = (int64_t)(page >= 0 ? page : any) * p.page_bytes + (int64_t)in_page * p.k_row +
-                                    pc.g * p.k_head;
-                a = p.kp + off;
-                b = p.vp + off;
+                return (int64_t)(page >= 0 ? page : any) * p.page_bytes + (int64_t)in_page * p.k_row + pc.g * p.k_head;
             };
             if constexpr (kGguf) {
 #pragma unroll
-                for (int c = 0; c < 4; ++c) at(c, id[c], rk[c], rv[c]);
+                for (int c = 0; c < 4; ++c) rec.k[c] = at(c, id[c]);
             } else {  // the wave's rows lie in one chunk
                 const int c = 4 * w / W;
                 int page = id[0];
 #pragma unroll
                 for (int i = 1; i < 4; ++i) page = c == i ? id[i] : page;
-                at(c, page, rk[0], rv[0]);
+                rec.k[0] = at(c, page);
             }
         }
     };
-    // row r of the tile -> the row of its chunk to read (every row read is a key of the item)
-    auto chunk_row = [&](int r) __attribute__((always_inline)) {
-        const int c = min(r >> 4, r_last >> 4);
-        const int x = c == (r_last >> 4) ? min(r & 15, r_last & 15) : (r & 15);
-        return c == 0 ? max(x, r_first) : x;
+    // row r of a tile -> the row of its 16-key chunk to read
+    auto chunk_row = [&](int r, const Rec& x) __attribute__((always_inline)) {
+        const int c = min(r >> 4, x.last >> 4);
+        const int y = c == (x.last >> 4) ? min(r & 15, x.last & 15) : (r & 15);
+        return c == 0 ? max(y, x.first) : y;
     };
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane(
         (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)&lds.tile[0][0][0]);
-    uint32_t raw[kGguf ? NBL : 1][kGguf ? NWD : 1];
-    auto load = [&](uint32_t slot) __attribute__((always_inline)) {  // the record's tile
-        if constexpr (!kGguf) {
-            const uint32_t dst = lds0 + slot * (2u * TILE) + 1024u * NTR * (uint32_t)w;
+    // offsets of this lane's rows in full tiles.  Row x of this wave's part, transfer i
+    auto part_row = [&](int i) __attribute__((always_inline)) { return kBN / W * w + i * (1024 / ROW) + lane / (D / 8); };
+    auto part_col = [&](int r) __attribute__((always_inline)) {
+        return 16u * (uint32_t)((lane % (D / 8)) ^ tile_swz<D>(r));
+    };
+    uint32_t off_k[kGguf ? 1 : NTR], off_v[SRC == TS_LOCAL ? NTR : 1];
+    if constexpr (!kGguf) {
 #pragma unroll
-            for (int i = 0; i < NTR; ++i) {
-                const int r = kBN / W * w + i * (1024 / ROW) + lane / (D / 8);
-                const uint32_t col = 16u * (uint32_t)((lane % (D / 8)) ^ tile_swz<D>(r));
-                uint32_t ko, vo;
-                if constexpr (SRC == TS_LOCAL) {
-                    const int x = max(min(r, r_last), r_first);
-                    ko = (uint32_t)x * (uint32_t)p.k_row;
-                    vo = (uint32_t)x * (uint32_t)p.v_row;
-                } else {
-                    ko = vo = (uint32_t)chunk_row(r) * (uint32_t)p.k_row;
-                }
-                dma16w(rk[0], ko + col, dst + 1024u * i);
-                dma16w(rv[0], vo + col, dst + TILE + 1024u * i);
-            }
-        } else {
+        for (int i = 0; i < NTR; ++i) {
+            const int r = part_row(i);  // (paged: r & 15, the same for K and V)
+            off_k[i] = (uint32_t)(SRC == TS_LOCAL ? r : r & 15) * (uint32_t)p.k_row + part_col(r);
+            if constexpr (SRC == TS_LOCAL) off_v[i] = (uint32_t)r * (uint32_t)p.v_row + part_col(r);
+        }
+    }
+    // this wave's part of K or V of a tile into LDS at dst
+    auto transfer = [&](bool is_v, const Rec& x, uint32_t dst) __attribute__((always_inline)) {
+        const uint64_t b64 = (uint64_t)(is_v ? p.vp + (SRC == TS_LOCAL ? x.v : x.k[0]) : p.kp + x.k[0]);
+        const uint8_t* base = (const uint8_t*)(((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(b64 >> 32)) << 32) |
+                                               (uint32_t)__builtin_amdgcn_readfirstlane((int)b64));
+        const bool own_v = SRC == TS_LOCAL && is_v;
+        dst += 1024u * NTR * (uint32_t)w;
+        if (x.first == 0 && x.last >= kBN - 1) {
+#pragma unroll
+            for (int i = 0; i < NTR; ++i)
+                dma16w(base, own_v ? off_v[SRC == TS_LOCAL ? i : 0] : off_k[kGguf ? 0 : i], dst + 1024u * i);
+            return;
+        }
+        const uint32_t step = (uint32_t)(own_v ? p.v_row : p.k_row);
+#pragma unroll
+        for (int i = 0; i < NTR; ++i) {
+            const int r = part_row(i);
+            const int y = SRC == TS_LOCAL ? max(min(r, x.last), x.first) : chunk_row(r, x);
+            dma16w(base, (uint32_t)y * step + part_col(r), dst + 1024u * i);
+        }
+    };
+    uint32_t blk_raw[kGguf ? NBL : 1][kGguf ? NWD : 1];
+    auto load_blocks = [&]() __attribute__((always_inline)) {  // GGUF: the record's tile into registers
+        if constexpr (kGguf) {
 #pragma unroll
             for (int i = 0; i < NBL; ++i) {
                 const int idx = i * 64 * W + tid;
-                if (NBL * 64 * W > 4 * D && idx >= 4 * D) break;
                 const bool is_v = idx >= 2 * D;
                 const int x = idx & (2 * D - 1), r = x / (D / 32), blk = x % (D / 32), c = r >> 4;
-                const uint8_t* base = is_v ? rv[0] : rk[0];
+                if (NBL * 64 * W > 4 * D && idx >= 4 * D) continue;
+                int64_t off = rec.k[0];
 #pragma unroll
-                for (int e = 1; e < 4; ++e) base = c == e ? (is_v ? rv[e] : rk[e]) : base;
+                for (int e = 1; e < NA; ++e) off = c == e ? rec.k[e] : off;
                 // from the block's 4-byte floor: an odd block starts 2 bytes past one; the
                 // last dword stays inside the entry
-                const uint32_t* s = reinterpret_cast<const uint32_t*>(base + (uint32_t)chunk_row(r) * (uint32_t)p.k_row +
+                const uint32_t row = (uint32_t)chunk_row(r, rec);
+                const uint32_t* s = reinterpret_cast<const uint32_t*>((is_v ? p.vp : p.kp) + off + row * (uint32_t)p.k_row +
                                                                       BE * blk - 2 * (blk & 1));
                 typedef uint32_t u32x4a __attribute__((ext_vector_type(4), aligned(4)));
 #pragma unroll
                 for (int e = 0; e + 4 <= NWD; e += 4) {
                     const u32x4a y = *reinterpret_cast<const u32x4a*>(s + e);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) raw[i][e + j] = y[j];
+                    for (int j = 0; j < 4; ++j) blk_raw[i][e + j] = y[j];
                 }
-                raw[i][NWD - 1] = s[NWD - 1];
+                blk_raw[i][NWD - 1] = s[NWD - 1];
             }
         }
     };
@@ -302,18 +349,18 @@ __global__ void __launch_bounds__(64 * W, 2) shared_tile_kernel(TileParams p) {
 #pragma unroll
             for (int i = 0; i < NBL; ++i) {
                 const int idx = i * 64 * W + tid;
-                if (NBL * 64 * W > 4 * D && idx >= 4 * D) break;
-                const int is_v = idx >= 2 * D;
+                const bool is_v = idx >= 2 * D;
                 const int x = idx & (2 * D - 1), r = x / (D / 32), blk = x % (D / 32);
+                if (NBL * 64 * W > 4 * D && idx >= 4 * D) continue;
                 const bool odd = (blk & 1) != 0;
                 uint32_t c[NWD - 1];
 #pragma unroll
                 for (int e = 0; e < NWD - 1; ++e)
-                    c[e] = odd ? raw[i][e + 1] : __builtin_amdgcn_alignbyte(raw[i][e + 1], raw[i][e], 2);
-                const uint16_t db = (uint16_t)(odd ? raw[i][0] >> 16 : raw[i][0] & 0xffffu);
+                    c[e] = odd ? blk_raw[i][e + 1] : __builtin_amdgcn_alignbyte(blk_raw[i][e + 1], blk_raw[i][e], 2);
+                const uint16_t db = (uint16_t)(odd ? blk_raw[i][0] >> 16 : blk_raw[i][0] & 0xffffu);
                 const _Float16 dh = __builtin_bit_cast(_Float16, db);
                 const f16x2 d2 = {dh, dh};
-                uint8_t* row = lds.tile[slot][is_v] + r * ROW;
+                uint8_t* row = lds.tile[slot][is_v ? 1 : 0] + r * ROW;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {  // chunk j: values 8j .. 8j + 7
                     u32x4 y;
@@ -327,6 +374,41 @@ __global__ void __launch_bounds__(64 * W, 2) shared_tile_kernel(TileParams p) {
                     }
                     *reinterpret_cast<u32x4*>(row + 16 * ((4 * blk + j) ^ tile_swz<D>(r))) = y;
                 }
+            }
+        }
+    };
+    // The V rows that this wave fetched of the tile in `slot`, one 16-key chunk, to fp16
+    auto convert = [&](uint32_t slot, int half) __attribute__((always_inline)) {
+        if constexpr (kConv) {
+            typedef uint16_t u16x2v __attribute__((ext_vector_type(2)));
+            uint32_t mx = 0;  // packed 16-bit maxima of the magnitudes
+            uint8_t* at = lds.tile[slot][1] + 1024u * NTR * (uint32_t)w + 16u * (uint32_t)lane;
+            u32x4 x[NTR];
+#pragma unroll
+            for (int i = 0; i < NTR; ++i) {
+                x[i] = *reinterpret_cast<const u32x4*>(at + 1024 * i);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    mx = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2v, mx),
+                                                                                __builtin_bit_cast(u16x2v, x[i][e] & 0x7fff7fffu)));
+            }
+            const uint32_t m = max(mx & 0xffffu, mx >> 16);
+            // 2^8 for values up to 255, 1 for larger ones, 2^20 where all are below 2^-12
+            const bool big = __ballot(m >= 0x4380u) != 0, tiny = __ballot(m >= 0x3980u) == 0;
+            // past 65504 (or no number), or all below 2^-33 but not 0: no scale fits
+            const bool bad = __ballot(m >= 0x4780u) != 0 || (__ballot(m >= 0x2f00u) == 0 && __ballot(m != 0) != 0);
+            const float scale = big ? 1.0f : tiny ? 1048576.0f : 256.0f;
+            if (lane == 0) lds.vexp[half][w] = bad ? __builtin_nanf("") : big ? 8.0f : tiny ? -12.0f : 0.0f;
+#pragma unroll
+            for (int i = 0; i < NTR; ++i) {
+                u32x4 y;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float f0 = bf16_bits_to_f32((uint16_t)(x[i][e] & 0xffffu)) * scale;
+                    const float f1 = bf16_bits_to_f32((uint16_t)(x[i][e] >> 16)) * scale;
+                    y[e] = (uint32_t)f32_to_f16_bits(f0) | ((uint32_t)f32_to_f16_bits(f1) << 16);
+                }
+                *reinterpret_cast<u32x4*>(at + 1024 * i) = y;
             }
         }
     };
@@ -355,36 +437,37 @@ __global__ void __launch_bounds__(64 * W, 2) shared_tile_kernel(TileParams p) {
     f32x16 o[D / 32];
     // reference max (log2 units): moves only when a score passes it by more than 8
     float m_run = 0.f, m_thr = 0.f, l_part = 0.f, csc = 0.f;
-    int lo = 0, hi = 0, hi_min = 0, nrow = 0;  // keys of this lane's row; the least hi of the wave; rows of the item
-    int64_t tok = 0;
-    int head = 0, seg_t0 = 0;
-    bool row_ok = false, active = false;
-    auto begin_item = [&]() __attribute__((always_inline)) {  // cc's, at tile cc.t
-        const int all = cc.d.ntok * p.G;
-        nrow = min(RB, all - RB * cc.rb);
-        seg_t0 = cc.t;
+    float v_base = 0.f;  // kConv: the largest vexp so far; o is 2^(8 - v_base) times the sums
+    int lo = 0, hi = 0, hi_min = 0;  // keys of this lane's row, the least end of the wave's rows
+    bool active = false;             // the wave has rows of the item
+
+    auto begin_item = [&]() __attribute__((always_inline)) {  // cc's
+        const auto* a = arg();
+        const SetDesc d = desc_of(cc.set);
+        const int G = a->G, nrow = min(RB, d.ntok * G - RB * cc.rb);
         active = 32 * w < nrow;
         if (!active) return;
         const int r = RB * cc.rb + min(32 * w + c32, nrow - 1);
-        row_ok = 32 * w + c32 < nrow;
-        tok = cc.d.row0 + r / p.G;
-        head = cc.g * p.G + r % p.G;
-        lo = cc.d.klo;
-        hi = cc.d.khi;
-        if (SRC != TS_LOCAL && cc.d.own == 0) hi = min(hi, p.seq_lens[tok]);
-        hi_min = hi;
-        if (SRC != TS_LOCAL && cc.d.own == 0) {
+        const int64_t tok = d.row0 + r / G;
+        const uint16_t* qp = a->q + tok * a->q_ts + (cc.g * G + r % G) * a->q_hs + 8 * h;
+        u32x4 x[D / 16];
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s) x[s] = *reinterpret_cast<const u32x4*>(qp + 16 * s);
+        lo = d.klo;
+        hi = hi_min = d.khi;
+        if (SRC != TS_LOCAL && d.own == 0) {
+            hi = min(hi, a->seq_lens[tok]);
+            hi_min = hi;
 #pragma unroll
             for (int m = 16; m >= 1; m >>= 1) hi_min = min(hi_min, __shfl_xor(hi_min, m, kWave));
             hi_min = __builtin_amdgcn_readfirstlane(hi_min);
         }
-        const uint16_t* qp = p.q + tok * p.q_ts + head * p.q_hs + 8 * h;
-        const float sl2 = p.scale * kLog2e;
+        const float sl2 = a->scale * kLog2e;
         csc = fabsf(sl2);
-        const uint32_t qflip = sl2 < 0.0f ? 0x80008000u : 0u;  // a negative scale flips Q's signs
-        u32x4 x[D / 16];
+        if (sl2 < 0.0f) {  // a negative scale flips Q's signs
 #pragma unroll
-        for (int s = 0; s < D / 16; ++s) x[s] = *reinterpret_cast<const u32x4*>(qp + 16 * s) ^ qflip;
+            for (int s = 0; s < D / 16; ++s) x[s] ^= 0x80008000u;
+        }
         if constexpr (kGguf && QBF) {
             // bf16 q in fp16: the row scaled by a power of two so that its largest
             // value is in 2^7 .. 2^8, which csc undoes
@@ -404,26 +487,32 @@ __global__ void __launch_bounds__(64 * W, 2) shared_tile_kernel(TileParams p) {
                     x[s][e] = (uint32_t)f32_to_f16_bits(bf16_bits_to_f32((uint16_t)(x[s][e] & 0xffffu)) * up) |
                               ((uint32_t)f32_to_f16_bits(bf16_bits_to_f32((uint16_t)(x[s][e] >> 16)) * up) << 16);
         }
+        // waited for here, before more transfers are issued: the compiler would wait for
+        // those too
 #pragma unroll
-        for (int s = 0; s < D / 16; ++s) qf[s] = as_v8<V8>(x[s]);
+        for (int s = 0; s < D / 16; ++s) {
+            asm volatile("" : "+v"(x[s]));
+            qf[s] = as_v8<V8>(x[s]);
+        }
 #pragma unroll
         for (int m = 0; m < D / 32; ++m)
 #pragma unroll
             for (int i = 0; i < 16; ++i) o[m][i] = 0.0f;
-        m_run = m_thr = -__builtin_inff();
+        m_run = m_thr = v_base = -__builtin_inff();
         l_part = 0.0f;
     };
 
-    auto process = [&](uint32_t slot, uint32_t valid) __attribute__((always_inline)) {
-        const int kt = (cc.d.klo & ~15) + kBN * cc.t;
+    // the tile in `slot`; valid: its 16-key chunks that hold keys; vexp: what weights of a
+    // chunk are scaled by, as powers of two (kConv)
+    auto process = [&](uint32_t slot, uint32_t valid, f32x4 vexp) __attribute__((always_inline)) {
+        const int kt = (cc.klo & ~15) + kBN * cc.t;
         const uint32_t k_slot = k_lane + slot * (2u * TILE);
-        const uint32_t v_slot[2] = {v_lane[0] + slot * (2u * TILE), v_lane[1] + slot * (2u * TILE)};
+        const uint32_t vbase[2] = {v_lane[0] + slot * (2u * TILE), v_lane[1] + slot * (2u * TILE)};
 #pragma unroll
         for (int r = 0; r < 2 / HB; ++r) {
             const int k0 = kt + 32 * HB * r;
             const uint32_t vb = HB == 2 ? valid : (valid >> (2 * r)) & 3u;
             if (vb == 0) continue;  // past the keys, or holes
-            const bool need_mask = k0 + 32 * HB > hi_min || k0 < lo || vb != (HB == 2 ? 15u : 3u);
             f32x16 sacc[HB];
 #pragma unroll
             for (int b = 0; b < HB; ++b)
@@ -450,14 +539,16 @@ __global__ void __launch_bounds__(64 * W, 2) shared_tile_kernel(TileParams p) {
                 for (int b = 0; b < HB; ++b) sacc[b] = M::mma(as_v8<V8>(ka[s % (KA + 1)][b]), qf[s], sacc[b]);
                 __builtin_amdgcn_sched_barrier(0);
             }
-            if (need_mask) {
+            if (k0 + 32 * HB > hi_min || k0 < lo || vb != (HB == 2 ? 15u : 3u)) {
+                asm volatile("");  // a branch: most tiles need none of this
+                const int up = hi - k0 - 4 * h, dn = lo - k0 - 4 * h;
 #pragma unroll
                 for (int b = 0; b < HB; ++b)
 #pragma unroll
                     for (int j = 0; j < 16; ++j) {
-                        const int kv = k0 + 32 * b + 8 * (j >> 2) + 4 * h + (j & 3);
+                        const int x = 32 * b + 8 * (j >> 2) + (j & 3);
                         const bool there = ((vb >> (2 * b + (j >> 3))) & 1) != 0;
-                        sacc[b][j] = kv < hi && kv >= lo && there ? sacc[b][j] : -__builtin_inff();
+                        sacc[b][j] = x < up && x >= dn && there ? sacc[b][j] : -__builtin_inff();
                     }
             }
             float mloc = sacc[0][0];
@@ -478,29 +569,50 @@ __global__ void __launch_bounds__(64 * W, 2) shared_tile_kernel(TileParams p) {
                     for (int i = 0; i < 16; ++i) o[m][i] *= alpha;
             }
             const float ref = m_run == -__builtin_inff() ? 0.0f : m_run - kOff;
+            if constexpr (kConv) {
+                const float top = fmaxf(fmaxf(vexp[0], vexp[1]), fmaxf(vexp[2], vexp[3]));
+                if (__builtin_amdgcn_readfirstlane(top > v_base)) {  // larger values than so far
+                    const float alpha = __builtin_amdgcn_exp2f(v_base - top);  // 0 from -inf
+                    v_base = top;
+#pragma unroll
+                    for (int m = 0; m < D / 32; ++m)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) o[m][i] *= alpha;
+                }
+            }
             u32x4 pt[2][2 * HB];  // [term][16-key chunk]
             float sum = 0.0f;
 #pragma unroll
-            for (int c = 0; c < 2 * HB; ++c)
+            for (int c = 0; c < 2 * HB; ++c) {
+                const float off = kConv ? (vexp[2 * HB * r + c] - v_base) - ref : -ref;
+                float part = 0.0f;
 #pragma unroll
                 for (int e = 0; e < 8; e += 2) {
                     const int j = 4 * (2 * (c & 1) + (e >> 2)) + (e & 3);
-                    const float x0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[c >> 1][j], csc, -ref));
-                    const float x1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[c >> 1][j + 1], csc, -ref));
-                    sum += x0 + x1;
-                    uint32_t t0, t1;
-                    two_terms<BF>(x0, x1, t0, t1);
-                    pt[0][c][e >> 1] = t0;
-                    pt[1][c][e >> 1] = t1;
+                    const float x0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[c >> 1][j], csc, off));
+                    const float x1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[c >> 1][j + 1], csc, off));
+                    part += x0 + x1;
+                    if constexpr (NT == 1) {
+                        pt[0][c][e >> 1] = (uint32_t)f32_to_half<PBF>(x0) | ((uint32_t)f32_to_half<PBF>(x1) << 16);
+                    } else {
+                        uint32_t t0, t1;
+                        two_terms<PBF>(x0, x1, t0, t1);
+                        pt[0][c][e >> 1] = t0;
+                        pt[1][c][e >> 1] = t1;
+                    }
                 }
-            l_part += sum;
+                sum += kConv ? part * __builtin_amdgcn_exp2f(v_base - vexp[2 * HB * r + c]) : part;
+            }
+            // O^T += V^T P^T
+            using MP = MT<PBF>;
+            using VP = typename MP::v8;
             u32x2 va[VA + 1][2];
             auto read_v = [&](int i) __attribute__((always_inline)) {
                 const int c = i / (D / 32), m = i % (D / 32);
                 const int vo = (2 * HB * r + c) * 16 * ROW + 256 * (m >> 2);
 #pragma unroll
                 for (int sec = 0; sec < 2; ++sec)
-                    va[i % (VA + 1)][sec] = lds_tr((v_slot[sec] ^ (uint32_t)(64 * (m & 3))) + (uint32_t)vo);
+                    va[i % (VA + 1)][sec] = lds_tr((vbase[sec] ^ (uint32_t)(64 * (m & 3))) + (uint32_t)vo);
             };
             constexpr int NV = 2 * HB * (D / 32);
 #pragma unroll
@@ -511,165 +623,192 @@ __global__ void __launch_bounds__(64 * W, 2) shared_tile_kernel(TileParams p) {
                 __builtin_amdgcn_sched_barrier(0);
                 const int c = i / (D / 32), m = i % (D / 32);
                 const u32x2* vi = va[i % (VA + 1)];
-                const V8 x = as_v8<V8>(u32x4{vi[0][0], vi[0][1], vi[1][0], vi[1][1]});
+                const VP x = as_v8<VP>(u32x4{vi[0][0], vi[0][1], vi[1][0], vi[1][1]});
 #pragma unroll
-                for (int u = 0; u < 2; ++u) o[m] = M::mma(x, as_v8<V8>(pt[u][c]), o[m]);
+                for (int u = 0; u < NT; ++u) o[m] = MP::mma(x, as_v8<VP>(pt[u][c]), o[m]);
                 __builtin_amdgcn_sched_barrier(0);
             }
+            l_part += sum;
         }
     };
 
-    // ---- the segment of cc's item that ends after tile t_end - 1
-    auto end_item = [&](int t_end) __attribute__((always_inline)) {
-        const bool cut = seg_t0 > 0 || t_end < cc.d.tiles;
+    bool bad_seen = false;
+    // ---- the segment (tiles t0 .. t1 - 1) of item (set, g, rb) ends
+    auto end_item = [&](int set, int g, int rb, int t0, int t1) __attribute__((always_inline)) {
+        const auto* a = arg();
+        const SetDesc d = desc_of(set);
+        const int G = a->G, nrow = min(RB, d.ntok * G - RB * rb);
+        const bool row_ok = 32 * w + c32 < nrow;
+        const bool cut = t0 > 0 || t1 < d.tiles;
         // partial row 0 of the segment (shared_plan.hpp)
-        const int64_t prow = p.paged ? plan_rows_paged(range, RB, p.Hq, p.G, p.total_rows, cc.d, cc.g, cc.rb)
-                                     : plan_rows_local(range, RB, seg_t0 > 0);
-        const bool direct = !p.paged && !cut;
+        const int64_t prow = a->paged ? plan_rows_paged(range, RB, a->Hq, G, a->total_rows, d.own, d.row0, d.ntok, g, rb)
+                                      : plan_rows_local(range, RB, t0 > 0);
+        const bool direct = !a->paged && !cut;
         const float l = l_part + shfl_xor(l_part, 32);
         bool bad = !(l == l);
 #pragma unroll
         for (int m = 0; m < D / 32; ++m)
 #pragma unroll
             for (int i = 0; i < 16; ++i) bad |= !(fabsf(o[m][i]) < __builtin_inff());
-        uint64_t badb = __ballot(bad && row_ok);
-        badb = (badb | (badb >> 32)) & 0xffffffffull;  // a row is the lane and its partner
-        if (row_ok && !((badb >> c32) & 1)) {
-            if (direct) {
-                const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-                uint16_t* op = p.out + (tok * p.Hq + head) * D + 4 * h;
+        bad_seen |= __ballot(bad && row_ok) != 0;
+        if (!row_ok) return;
+        const float vs = kConv ? __builtin_amdgcn_exp2f(v_base - 8.0f) : 1.0f;
+        if (direct) {
+            const int r = RB * rb + 32 * w + c32;
+            const float inv = l > 0.0f ? vs / l : 0.0f;
+            uint16_t* op = a->out + ((int64_t)(d.row0 + r / G) * a->Hq + g * G + r % G) * D + 4 * h;
 #pragma unroll
-                for (int m = 0; m < D / 32; ++m)
+            for (int m = 0; m < D / 32; ++m)
 #pragma unroll
-                    for (int b = 0; b < 4; ++b) {
-                        uint32_t x[2];
+                for (int b = 0; b < 4; ++b) {
+                    uint32_t x[2];
 #pragma unroll
-                        for (int i = 0; i < 2; ++i)
-                            x[i] = (uint32_t)f32_to_half<QBF>(o[m][4 * b + 2 * i] * inv) |
-                                   ((uint32_t)f32_to_half<QBF>(o[m][4 * b + 2 * i + 1] * inv) << 16);
-                        *reinterpret_cast<u32x2*>(op + 32 * m + 8 * b) = u32x2{x[0], x[1]};
-                    }
-            } else {
-                float* pp = p.part + (prow + 32 * w + c32) * (D + 4);
-#pragma unroll
-                for (int m = 0; m < D / 32; ++m)
-#pragma unroll
-                    for (int b = 0; b < 4; ++b)
-                        *reinterpret_cast<f32x4*>(pp + 32 * m + 8 * b + 4 * h) =
-                            f32x4{o[m][4 * b], o[m][4 * b + 1], o[m][4 * b + 2], o[m][4 * b + 3]};
-                // o and l hold weights of 2^(s - m_run + kOff): the reference they go with
-                if (h == 0) *reinterpret_cast<float2*>(pp + D) = make_float2(m_run - kOff, l);
-            }
-        }
-        while (badb) {
-            const int c = (int)__builtin_ctzll(badb);
-            badb &= badb - 1;
-            const int r = RB * cc.rb + 32 * w + c;
-            const int64_t t = cc.d.row0 + r / p.G;
-            const int hd = cc.g * p.G + r % p.G, kb = cc.d.klo & ~15;
-            const int k0 = max(cc.d.klo, kb + kBN * seg_t0);
-            const int k1 = min(__builtin_amdgcn_readlane(hi, c), kb + kBN * t_end);
-            const int64_t koff = cc.g * p.k_head + (p.paged ? 0 : cc.d.src * p.k_row);
-            const int64_t voff = cc.g * p.v_head + (p.paged ? 0 : cc.d.src * p.v_row);
-            shared_row_exact<D, SRC, QBF>(p.q + t * p.q_ts + hd * p.q_hs, p.kp + koff, p.vp + voff, p.k_row, p.v_row,
-                                          p.bt + (p.paged ? cc.d.src * p.max_blocks : 0), p.page_bytes, p.bs, p.scale,
-                                          k0, k1, lds.qs[w],
-                                          direct ? p.out + (t * p.Hq + hd) * D : nullptr,
-                                          direct ? nullptr : p.part + (prow + 32 * w + c) * (D + 4));
-        }
-    };
-
-    if (p.whole && units == 0) {  // rows of a sequence without states
-        begin_item();
-        if (active) {
+                    for (int i = 0; i < 2; ++i)
+                        x[i] = (uint32_t)f32_to_half<QBF>(o[m][4 * b + 2 * i] * inv) |
+                               ((uint32_t)f32_to_half<QBF>(o[m][4 * b + 2 * i + 1] * inv) << 16);
+                    *reinterpret_cast<u32x2*>(op + 32 * m + 8 * b) = u32x2{x[0], x[1]};
+                }
+        } else {
+            float* pp = a->part + (prow + 32 * w + c32) * (D + 4);
 #pragma unroll
             for (int m = 0; m < D / 32; ++m)
 #pragma unroll
                 for (int b = 0; b < 4; ++b)
-                    if (row_ok)
-                        *reinterpret_cast<u32x2*>(p.out + (tok * p.Hq + head) * D + 4 * h + 32 * m + 8 * b) = u32x2{0u, 0u};
+                    *reinterpret_cast<f32x4*>(pp + 32 * m + 8 * b + 4 * h) =
+                        f32x4{o[m][4 * b], o[m][4 * b + 1], o[m][4 * b + 2], o[m][4 * b + 3]} * vs;
+            // o and l hold weights of 2^(s - m_run + kOff): the reference they go with
+            if (h == 0) *reinterpret_cast<float2*>(pp + D) = make_float2(m_run - kOff, l);
+        }
+    };
+    // Rows whose sums met an infinity or a NaN (a product takes every key's V times its
+    // weight, also where that is 0) go key by key.  After the range, so that the
+    // call has nothing of the loop's to keep: its segments are walked again, and the
+    // rows in question known by what was written
+    auto rerun = [&](Cursor c, int n) __attribute__((always_inline)) {
+        const auto* a = arg();
+        while (n > 0) {
+            const SetDesc d = desc_of(c.set);
+            const int G = a->G, nrow = min(RB, d.ntok * G - RB * c.rb), t0 = c.t, t1 = min(d.tiles, t0 + n);
+            const bool direct = !a->paged && t0 == 0 && t1 == d.tiles;
+            const int64_t prow = a->paged ? plan_rows_paged(range, RB, a->Hq, G, a->total_rows, d.own, d.row0, d.ntok, c.g, c.rb)
+                                          : plan_rows_local(range, RB, t0 > 0);
+            for (int i = 32 * w; i < min(32 * w + 32, nrow); ++i) {
+                const int r = RB * c.rb + i, hd = c.g * G + r % G, kb = d.klo & ~15;
+                const int64_t t = d.row0 + r / G;
+                uint16_t* op = a->out + (t * a->Hq + hd) * D;
+                float* pp = a->part + (prow + i) * (D + 4);
+                bool bad = false;
+#pragma unroll
+                for (int k = 0; k < D / 64; ++k) {
+                    const float x = direct ? half_to_f32<QBF>(__builtin_nontemporal_load(op + lane + 64 * k))
+                                           : __builtin_nontemporal_load(pp + lane + 64 * k);
+                    bad |= !(fabsf(x) < __builtin_inff());
+                }
+                if (!direct) bad |= !(__builtin_nontemporal_load(pp + D + 1) < __builtin_inff());
+                if (__ballot(bad) == 0) continue;
+                int k1 = min(d.khi, kb + kBN * t1);
+                if (SRC != TS_LOCAL && d.own == 0) k1 = min(k1, a->seq_lens[t]);
+                const int64_t koff = c.g * a->k_head + (a->paged ? 0 : d.src * a->k_row);
+                const int64_t voff = c.g * a->v_head + (a->paged ? 0 : d.src * a->v_row);
+                shared_row_exact<D, SRC, QBF>(a->q + t * a->q_ts + hd * a->q_hs, a->kp + koff, a->vp + voff, a->k_row,
+                                              a->v_row, a->bt + (a->paged ? d.src * a->max_blocks : 0), a->page_bytes,
+                                              a->bs, a->scale, max(d.klo, kb + kBN * t0), k1, lds.qs[w],
+                                              direct ? op : nullptr, direct ? nullptr : pp);
+            }
+            n -= t1 - t0;
+            if (n <= 0) break;
+            c.t = d.tiles - 1;
+            c.tiles = d.tiles;
+            advance(c);
+        }
+    };
+
+    if (units == 0) {  // (whole items) rows of a sequence without states
+        const auto* a = arg();
+        const SetDesc d = desc_of(cc.set);
+        const int nrow = min(RB, d.ntok * a->G - RB * cc.rb);
+        for (int i = tid; i < nrow * (D / 8); i += 64 * W) {
+            const int r = RB * cc.rb + i / (D / 8);
+            *reinterpret_cast<u32x4*>(a->out + ((int64_t)(d.row0 + r / a->G) * a->Hq + cc.g * a->G + r % a->G) * D +
+                                      8 * (i % (D / 8))) = u32x4{0u, 0u, 0u, 0u};
         }
         return;
     }
 
-    int fetched = 0, loaded = 0;  // tiles
-    auto next_record = [&]() __attribute__((always_inline)) {
-        if (fetched == units) return;
-        if (fetched) advance(pc);
-        fetch();
-        ++fetched;
-    };
-    auto load_next = [&](uint32_t slot) __attribute__((always_inline)) {
-        load(slot);
-        vq = (vq << 4) | r_valid;
+    const Cursor start = cc;
+    int loaded = 0, seg_t0 = cc.t;
+    auto load = [&](uint32_t slot) __attribute__((always_inline)) {  // the record's tile
+        if constexpr (kGguf) {
+            load_blocks();
+        } else {
+            transfer(false, rec, lds0 + slot * (2u * TILE));
+            transfer(true, rec, lds0 + slot * (2u * TILE) + TILE);
+        }
         ++loaded;
+        fetch();
     };
-    next_record();
-    if constexpr (kGguf) {
-        load_next(0);
-        next_record();
-        uint32_t slot = 0;
-        for (int u = 0; u < units; ++u) {
-            stage(slot);
-            const uint32_t valid = vq & 15u;
-            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            if (loaded < units) {
-                load_next(0);
-                next_record();
-            }
-            if (u == 0 || cc.t == 0) begin_item();
-            if (active) process(slot, valid);
-            if (active && (cc.t + 1 == cc.d.tiles || u + 1 == units)) end_item(cc.t + 1);
-            if (u + 1 < units) advance(cc);
-            slot ^= 1;
-        }
-    } else {
-        // tile u in slot u % NS, the next NS - 1 in flight while it runs.  The barrier
-        // makes tile u visible and shows slot (u - 1) % NS free, which then receives
-        // tile u + NS - 1 (2 NTR transfers a tile and wave; vmcnt retires in order)
-        load_next(0);
-        next_record();
-        if (NS == 3 && loaded < units) {
-            load_next(1);
-            next_record();
-        }
-        uint32_t slot = 0, fill = NS - 1;
-        for (int u = 0; u < units; ++u) {
+    auto landed = [&](int u) __attribute__((always_inline)) {  // this wave's part of tile u
+        if constexpr (!kGguf) {  // (vmcnt retires in order)
             if (NS == 3 && loaded > u + 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * NTR) : "memory");
             else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            if (loaded < units) {
-                load_next(fill);
-                next_record();
-            }
-            if (u == 0 || cc.t == 0) begin_item();
-            const uint32_t valid = (vq >> (4 * (loaded - u - 1))) & 15u;
-            if (active) process(slot, valid);
-            if (active && (cc.t + 1 == cc.d.tiles || u + 1 == units)) end_item(cc.t + 1);
-            if (u + 1 < units) advance(cc);
-            slot = slot == NS - 1 ? 0 : slot + 1;
-            fill = fill == NS - 1 ? 0 : fill + 1;
         }
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    };
+    // Tile u in slot u % NS, the next NS - 1 in flight while it runs (GGUF: the next in
+    // registers).  The barrier makes tile u visible and shows slot (u - 1) % NS
+    // free, which then receives tile u + NS - 1.
+    fetch();
+    load(0);
+    if (!kGguf && NS == 3 && loaded < units) load(1);
+    if constexpr (kConv) {
+        landed(0);
+        convert(0, 0);
     }
+    uint32_t slot = 0, fill = NS - 1;
+    for (int u = 0; u < units; ++u) {
+        if constexpr (kGguf) stage(slot);
+        else if constexpr (!kConv) landed(u);
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (u == 0 || cc.t == 0) begin_item();
+        const uint32_t valid = (vq >> (4 * (fetched - 1 - u))) & 15u;
+        if (loaded < units) load(fill);
+        f32x4 vexp = {0.0f, 0.0f, 0.0f, 0.0f};
+        if constexpr (kConv) vexp = *reinterpret_cast<const f32x4*>(lds.vexp[u & 1]);
+        if (active) process(slot, valid, vexp);
+        const bool more = u + 1 < units, ends = cc.t + 1 == cc.tiles || !more;
+        if (ends && active) end_item(cc.set, cc.g, cc.rb, seg_t0, cc.t + 1);
+        slot = slot == NS - 1 ? 0 : slot + 1;
+        fill = fill == NS - 1 ? 0 : fill + 1;
+        if (more) {
+            advance(cc);
+            if (ends) seg_t0 = cc.t;
+            if constexpr (kConv) {
+                landed(u + 1);
+                convert(slot, (u + 1) & 1);
+            }
+        }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (bad_seen) rerun(start, units);
 }
 
-template <int D, int SRC, bool QBF, int W>
+template <int D, int SRC, bool QBF, bool CONV = false>
 int launch_tile(const TileParams& p, unsigned grid, hipStream_t s) {
-    hipLaunchKernelGGL((shared_tile_kernel<D, SRC, QBF, W>), dim3(grid), dim3(64 * W), 0, s, p);
+    hipLaunchKernelGGL((shared_tile_kernel<D, SRC, QBF, CONV>), dim3(grid), dim3(64 * kTileWaves), 0, s, p);
     VMC_LAUNCH_CHECK();
     return VMC_OK;
 }
 
 template <int D>
-int dispatch_tile(const TileParams& p, int src, bool qbf, int waves, unsigned grid, hipStream_t s) {
+int dispatch_tile(const TileParams& p, int src, bool qbf, bool conv, unsigned grid, hipStream_t s) {
     switch (src) {
         case TS_LOCAL:
-            if (waves == 8) return qbf ? launch_tile<D, TS_LOCAL, true, 8>(p, grid, s) : launch_tile<D, TS_LOCAL, false, 8>(p, grid, s);
-            return qbf ? launch_tile<D, TS_LOCAL, true, 4>(p, grid, s) : launch_tile<D, TS_LOCAL, false, 4>(p, grid, s);
-        case TS_PAGED: return qbf ? launch_tile<D, TS_PAGED, true, 4>(p, grid, s) : launch_tile<D, TS_PAGED, false, 4>(p, grid, s);
-        case TS_Q8: return qbf ? launch_tile<D, TS_Q8, true, 4>(p, grid, s) : launch_tile<D, TS_Q8, false, 4>(p, grid, s);
-        case TS_Q4: return qbf ? launch_tile<D, TS_Q4, true, 4>(p, grid, s) : launch_tile<D, TS_Q4, false, 4>(p, grid, s);
+            if (!qbf) return launch_tile<D, TS_LOCAL, false>(p, grid, s);
+            return conv ? launch_tile<D, TS_LOCAL, true, true>(p, grid, s) : launch_tile<D, TS_LOCAL, true>(p, grid, s);
+        case TS_PAGED:
+            if (!qbf) return launch_tile<D, TS_PAGED, false>(p, grid, s);
+            return conv ? launch_tile<D, TS_PAGED, true, true>(p, grid, s) : launch_tile<D, TS_PAGED, true>(p, grid, s);
+        case TS_Q8: return qbf ? launch_tile<D, TS_Q8, true>(p, grid, s) : launch_tile<D, TS_Q8, false>(p, grid, s);
+        case TS_Q4: return qbf ? launch_tile<D, TS_Q4, true>(p, grid, s) : launch_tile<D, TS_Q4, false>(p, grid, s);
         default: return VMC_EINVAL;
     }
 }

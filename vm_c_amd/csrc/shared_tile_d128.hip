@@ -3,8 +3,8 @@
 
 namespace vmc {
 
-int shared_tile_d128(const TileParams& p, int src, bool q_bf16, int waves, unsigned grid, hipStream_t s) {
-    return dispatch_tile<128>(p, src, q_bf16, waves, grid, s);
+int shared_tile_d128(const TileParams& p, int src, bool q_bf16, bool conv, unsigned grid, hipStream_t s) {
+    return dispatch_tile<128>(p, src, q_bf16, conv, grid, s);
 }
 
 }  // namespace vmc
