@@ -196,3 +196,12 @@ def test_value_magnitudes(dev, d, t, size):
         else:
             v *= float(size)
     Cross(dev, [t, t], [130, 70], (8, 2), d, "bf16", seed=10, edit=edit).check(mixed=True)
+
+
+# more sequences than the plan holds in LDS
+@pytest.mark.parametrize("d", [64, 256])
+def test_a_thousand_sequences(dev, d):
+    rng = np.random.default_rng(d)
+    n = rng.integers(0, 20, 1500)
+    n[700] = 3000
+    Cross(dev, rng.integers(0, 3, 1500), n, (4, 2), d, "f16", seed=11, gap=(3, 2)).check()

@@ -243,3 +243,15 @@ def test_scores_far_apart(dev, d):
         k[b.slots(1)[100]] *= 30
     b = Batch(dev, [90, 120, 200, 64], [(4, 64)], (8, 2), d, F16, "f16", seed=7, edit=edit, scale=1.0)
     b.check()
+
+
+# more rows, and more groups, than the plan holds in LDS
+@pytest.mark.parametrize("d", [64, 256])
+def test_a_thousand_rows(dev, d):
+    rng = np.random.default_rng(d)
+    lens = rng.integers(0, 60, 1300)
+    groups = [(int(n), int(s)) for n, s in zip(rng.integers(0, 4, 600), rng.integers(0, 50, 600))]
+    while sum(g[0] for g in groups) > 1290:
+        groups.pop()
+    lens[5] = 4000
+    Batch(dev, lens, groups, (4, 2), d, F16, "f16", seed=12, lead=7).check()

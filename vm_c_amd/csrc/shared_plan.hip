@@ -16,175 +16,258 @@ namespace {
 
 constexpr int kPlanThreads = 1024;
 constexpr int kUnitsMin = kItemCost + 1;  // fewest units of a range: one tile
-constexpr int kPlanCached = 1024;  // sets that the plan keeps in LDS
+constexpr int kPlanCached = 1024;         // sets, and ranges, that the short plan holds in LDS
 
-// Inclusive scan over the workgroup of N values a thread by op; all: the last one's.
-template <int N, typename T, typename Op>
-__device__ __forceinline__ void block_incl_scan(T (&v)[N], T (*sh)[N], Op op, T (&all)[N]) {
+// Inclusive scan over the wave in six DPP steps (row_shr 1, 2, 4, 8, then the last lane of
+// the row before, then lane 31); op(v, 0) = v for the values scanned
+template <typename Op>
+__device__ __forceinline__ int wave_scan(int v, Op op) {
+    v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true));
+    v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true));
+    v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true));
+    v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true));
+    v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false));
+    v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false));
+    return v;
+}
+// over the workgroup (16 waves at most; sh: 16 entries); all: the last one's
+template <typename Op>
+__device__ __forceinline__ int block_scan(int v, int* sh, Op op, int& all) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, nw = blockDim.x >> 6;
+    v = wave_scan(v, op);
+    if (lane == 63) sh[w] = v;
+    __syncthreads();
+    int x[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = sh[i];
+    int run = 0, before = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        before = i < w ? op(run, x[i]) : before;
+        run = i < nw ? op(run, x[i]) : run;
+    }
+    all = run;
+    __syncthreads();
+    return op(v, before);
+}
+__device__ __forceinline__ long long block_scan(long long v, long long* sh, long long& all) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, nw = blockDim.x >> 6;
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1)
-#pragma unroll
-        for (int k = 0; k < N; ++k) {
-            const T o = __shfl_up(v[k], d, kWave);
-            if (lane >= d) v[k] = op(v[k], o);
-        }
-    if (lane == 63)
-#pragma unroll
-        for (int k = 0; k < N; ++k) sh[w][k] = v[k];
+    for (int d = 1; d < 64; d <<= 1) {
+        const long long o = __shfl_up(v, d, kWave);
+        if (lane >= d) v += o;
+    }
+    if (lane == 63) sh[w] = v;
     __syncthreads();
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-        T run = sh[0][k], before = run;
-        for (int i = 1; i < nw; ++i) {
-            if (i == w) before = run;
-            run = op(run, sh[i][k]);
-        }
-        if (w > 0) v[k] = op(before, v[k]);
-        all[k] = run;
+    long long before = 0;
+    all = 0;
+    for (int i = 0; i < nw; ++i) {
+        before += i < w ? sh[i] : 0;
+        all += sh[i];
     }
     __syncthreads();
+    return v + before;
 }
 
-__device__ __forceinline__ int64_t div_small(int64_t x, int64_t y) {  // x, y >= 0; y > 0
-    return ((x | y) >> 32) == 0 ? (int64_t)((uint32_t)x / (uint32_t)y) : x / y;
+template <typename T>
+__device__ __forceinline__ T div_floor(T x, T y) {  // x >= 0, y > 0
+    if constexpr (sizeof(T) == 4) return (T)((uint32_t)x / (uint32_t)y);
+    else return ((x | y) >> 32) == 0 ? (T)((uint32_t)x / (uint32_t)y) : x / y;
 }
 
-// tiles before unit u of a set (with the first tile's place at or after u in *rec)
-__device__ __forceinline__ int64_t tiles_before(const SetDesc& d, int64_t cum, int64_t cumt, int64_t u, RangeRec* rec) {
-    const int64_t rem = u - cum;
-    const int per = d.tiles + kItemCost;
-    const int64_t item = div_small(rem, per);
-    const int x = max((int)(rem - item * per) - kItemCost, 0);
-    if (rec) {
-        rec->g = (int)div_small(item, d.nb);
-        rec->rb = (int)(item - (int64_t)rec->g * d.nb);
-        rec->t = x;
+// One set, from its length (group: shared tokens; sequence: states; row: tokens)
+__device__ __forceinline__ SetDesc make_desc(const PlanParams& p, int i, int row0, int ntok, int len, int key0, int group,
+                                             int shared) {
+    SetDesc d = {};
+    if (i < p.ns) {
+        d.row0 = row0;
+        d.ntok = ntok;
+        const int n = max(len, 0);
+        if (p.paged) {
+            d.src = row0;
+            // a group of one row has nothing to share: all its keys are the row's own
+            d.khi = ntok > 1 ? min(n, p.max_keys) : 0;
+        } else {
+            const long long end = min((long long)key0 + n, (long long)p.num_keys);
+            d.src = max(key0, 0);
+            d.khi = (int)max(end - d.src, 0ll);
+        }
+    } else {
+        d.row0 = d.src = i - p.ns;
+        d.ntok = 1;
+        d.khi = min(len, p.max_keys);
+        d.klo = max(shared, 0);
+        d.own = group + 2;  // 1: of no group
     }
-    return cumt + item * d.tiles + x;
+    d.nb = (int)div_floor<long long>((long long)d.ntok * p.G + p.RB - 1, p.RB);
+    d.tiles = d.ntok > 0 && d.khi > d.klo ? (int)(((long long)d.khi - (d.klo & ~15) + 63) / 64) : 0;
+    return d;
+}
+// the group of a row that shares something with others, or -1: starts gs[0 .. ns]
+__device__ __forceinline__ int group_of(const int* gs, int ns, int row) {
+    int lo = 0, hi = ns + 1;  // starts that are <= row
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (gs[mid] <= row) lo = mid + 1;
+        else hi = mid;
+    }
+    return lo >= 1 && lo <= ns && gs[lo] - gs[lo - 1] > 1 ? lo - 1 : -1;
+}
+// tiles before unit u of a set (and the first tile's place at or after u)
+template <typename T>
+__device__ __forceinline__ T tiles_before(const SetDesc& d, T cum, T cumt, T u, RangeRec& rec) {
+    const T rem = u - cum, per = d.tiles + kItemCost, item = div_floor<T>(rem, per);
+    rec.t = max((int)(rem - item * per) - kItemCost, 0);
+    rec.g = (int)div_floor<T>(item, d.nb);
+    rec.rb = (int)(item - (T)rec.g * d.nb);
+    return cumt + item * d.tiles + rec.t;
+}
+// last set of n with cum <= u
+template <typename T>
+__device__ __forceinline__ int set_of(const T* cum, int n, T u) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (cum[mid] <= u) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+__device__ __forceinline__ RowRec make_row(const SetDesc& own, int64_t own_u, const SetDesc* desc, int64_t grp_u) {
+    RowRec r = {};
+    r.own_u = own_u;
+    r.own_tiles = own.tiles;
+    if (own.own > 1) {
+        const SetDesc d = desc[own.own - 2];
+        r.grp_u = grp_u;
+        r.grp_tiles = d.tiles;
+        r.grp_nb = d.nb;
+        r.grp_row0 = d.row0;
+        r.grp_ntok = d.ntok;
+    }
+    return r;
 }
 
-// CACHED: the sets fit the LDS copies, which later steps of the plan read instead of
-// what it has just written
-template <bool CACHED>
+// The plan of a call of at most kPlanCached sets and ranges whose units fit 32 bits, a
+// thread a set: every step from registers and LDS.  What bounds it: its chain of
+// dependent steps.
 __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(PlanParams p) {
-    constexpr int NC = CACHED ? kPlanCached : 1;
-    __shared__ int shi[kPlanThreads / 64][1];
-    __shared__ long long shl[kPlanThreads / 64][2];
-    __shared__ long long s_cum[NC + 1], s_cumt[NC + 1];
-    __shared__ SetDesc s_desc[NC];
-    __shared__ int s_gs[NC + 1];
-    const int tid = threadIdx.x, nt = blockDim.x;
-    // lengths of this thread's first set: on their way while the starts are scanned
+    __shared__ int sh[3][16];
+    __shared__ int s_gs[kPlanCached + 1], s_len[kPlanCached], s_cum[kPlanCached + 1], s_cumt[kPlanCached + 1];
+    __shared__ int s_first[kPlanCached + 1];  // tiles before each range
+    __shared__ SetDesc s_desc[kPlanCached];
+    const int i = threadIdx.x;
     int len = 0, key0 = 0;
-    auto lengths = [&](int i) {
-        if (i < p.ns) {
-            len = p.set_lens[i];
-            if (!p.paged) key0 = p.key_starts[i];
-        } else if (i < p.nsets) {
-            len = p.seq_lens[i - p.ns];
-        }
-    };
-    lengths(tid);
+    if (i < p.ns) {
+        len = p.set_lens[i];
+        if (!p.paged) key0 = p.key_starts[i];
+    } else if (i < p.nsets) {
+        len = p.seq_lens[i - p.ns];
+    }
+    int all;
+    const int start = p.ns > 0 && i <= p.ns ? min(max(p.starts[i], 0), p.rows) : 0;
+    const int gs = block_scan(start, sh[0], [](int a, int b) { return max(a, b); }, all);
+    if (i <= p.ns) {
+        s_gs[i] = gs;
+        p.gs[i] = gs;
+    }
+    if (i < p.nsets) s_len[i] = len;
+    __syncthreads();
+    SetDesc d = {};
+    int units = 0, tiles = 0;
+    if (i < p.nsets) {
+        const int j = i < p.ns ? -1 : group_of(s_gs, p.ns, i - p.ns);
+        d = make_desc(p, i, i < p.ns ? s_gs[i] : 0, i < p.ns ? s_gs[i + 1] - s_gs[i] : 0, len, key0, j, j >= 0 ? s_len[j] : 0);
+        const int items = p.Hkv * d.nb;
+        units = p.whole ? items : d.tiles ? items * (d.tiles + kItemCost) : 0;
+        tiles = items * d.tiles;
+        p.desc[i] = d;
+        s_desc[i] = d;
+    }
+    int total, total_t;
+    const int cum = block_scan(units, sh[1], [](int a, int b) { return a + b; }, total) - units;
+    const int cumt = block_scan(tiles, sh[2], [](int a, int b) { return a + b; }, total_t) - tiles;
+    if (i < p.nsets) {
+        p.cum[i] = cum;
+        s_cum[i] = cum;
+        s_cumt[i] = cumt;
+    }
+    if (i == 0) p.cum[p.nsets] = total;
+    if (p.whole) return;
+    __syncthreads();
+    const int n = plan_ranges(total, p.grid, p.umin);
+    RangeRec r = {};
+    if (i < n) {
+        const int u = (int)div_floor<long long>((long long)i * total, n);
+        r.set = set_of(s_cum, p.nsets, u);
+        r.d = s_desc[r.set];
+        r.ntiles = tiles_before(r.d, s_cum[r.set], s_cumt[r.set], u, r);
+        s_first[i] = r.ntiles;
+    }
+    if (i == 0) s_first[n] = total_t;
+    __syncthreads();
+    if (i < n) r.ntiles = s_first[i + 1] - r.ntiles;
+    if (i < p.grid) p.range[i] = r;
+    if (p.paged && i >= p.ns && i < p.nsets)
+        p.row[i - p.ns] = make_row(d, cum, s_desc, d.own > 1 ? s_cum[d.own - 2] : 0);
+}
+
+// The plan of any other call, through memory
+__global__ void __launch_bounds__(kPlanThreads) shared_plan_long_kernel(PlanParams p) {
+    __shared__ int shi[16];
+    __shared__ long long shl[16];
+    const int tid = threadIdx.x, nt = blockDim.x;
     int carry = 0;
     for (int i0 = 0; i0 <= p.ns; i0 += nt) {
         const int i = i0 + tid;
-        int v[1] = {p.ns > 0 && i <= p.ns ? min(max(p.starts[i], 0), p.rows) : 0};
-        int all[1];
-        block_incl_scan<1>(v, shi, [](int a, int b) { return max(a, b); }, all);
-        if (i <= p.ns) {
-            p.gs[i] = max(carry, v[0]);
-            if (CACHED) s_gs[i] = max(carry, v[0]);
-        }
-        carry = max(carry, all[0]);
+        int all;
+        const int v = block_scan(p.ns > 0 && i <= p.ns ? min(max(p.starts[i], 0), p.rows) : 0, shi,
+                                 [](int a, int b) { return max(a, b); }, all);
+        if (i <= p.ns) p.gs[i] = max(carry, v);
+        carry = max(carry, all);
     }
     __syncthreads();
-    const int* gs = CACHED ? s_gs : p.gs;
-    long long done[2] = {0, 0};  // units, tiles
+    long long total = 0, total_t = 0;
     for (int i0 = 0; i0 < p.nsets; i0 += nt) {
         const int i = i0 + tid;
-        if (i0) lengths(i);
-        SetDesc d = {};
-        long long amount[2] = {0, 0};
+        long long units = 0, tiles = 0;
         if (i < p.nsets) {
+            SetDesc d;
             if (i < p.ns) {
-                d.row0 = gs[i];
-                d.ntok = gs[i + 1] - d.row0;
-                const int n = max(len, 0);
-                if (p.paged) {
-                    d.src = d.row0;
-                    // a group of one row has nothing to share: all its keys are the row's own
-                    d.khi = d.ntok > 1 ? min(n, p.max_keys) : 0;
-                } else {
-                    const long long end = min((long long)key0 + n, (long long)p.num_keys);
-                    d.src = max(key0, 0);
-                    d.khi = (int)max(end - d.src, 0ll);
-                }
+                d = make_desc(p, i, p.gs[i], p.gs[i + 1] - p.gs[i], p.set_lens[i], p.paged ? 0 : p.key_starts[i], -1, 0);
             } else {
-                d.row0 = d.src = i - p.ns;
-                d.ntok = 1;
-                d.khi = min(len, p.max_keys);
-                int lo = 0, hi = p.ns + 1;  // starts that are <= row
-                while (lo < hi) {
-                    const int mid = (lo + hi) >> 1;
-                    if (gs[mid] <= d.row0) lo = mid + 1;
-                    else hi = mid;
-                }
-                const bool in = lo >= 1 && lo <= p.ns && gs[lo] - gs[lo - 1] > 1;
-                if (in) d.klo = max(p.set_lens[lo - 1], 0);
-                d.own = in ? lo + 1 : 1;  // 2 + its group
+                const int j = group_of(p.gs, p.ns, i - p.ns);
+                d = make_desc(p, i, 0, 0, p.seq_lens[i - p.ns], 0, j, j >= 0 ? p.set_lens[j] : 0);
             }
-            d.nb = (int)div_small((long long)d.ntok * p.G + p.RB - 1, p.RB);
-            d.tiles = d.ntok > 0 && d.khi > d.klo ? (int)(((long long)d.khi - (d.klo & ~15) + 63) / 64) : 0;
             const long long items = (long long)p.Hkv * d.nb;
-            amount[0] = p.whole ? items : d.tiles ? items * (d.tiles + kItemCost) : 0;
-            amount[1] = items * d.tiles;
+            units = p.whole ? items : d.tiles ? items * (d.tiles + kItemCost) : 0;
+            tiles = items * d.tiles;
             p.desc[i] = d;
-            if (CACHED) s_desc[i] = d;
         }
-        long long incl[2] = {amount[0], amount[1]}, all[2];
-        block_incl_scan<2>(incl, shl, [](long long a, long long b) { return a + b; }, all);
+        long long all, all_t;
+        const long long cum = block_scan(units, shl, all) - units, cumt = block_scan(tiles, shl, all_t) - tiles;
         if (i < p.nsets) {
-            const long long u = done[0] + incl[0] - amount[0], v = done[1] + incl[1] - amount[1];
-            p.cum[i] = u;
-            if (CACHED) {
-                s_cum[i] = u;
-                s_cumt[i] = v;
-            } else {
-                p.cumt[i] = v;
-            }
+            p.cum[i] = total + cum;
+            p.cumt[i] = total_t + cumt;
         }
-        done[0] += all[0];
-        done[1] += all[1];
+        total += all;
+        total_t += all_t;
     }
-    if (tid == 0) p.cum[p.nsets] = done[0];
+    if (tid == 0) p.cum[p.nsets] = total;
     if (p.whole) return;
     __syncthreads();
-    const long long* cum = CACHED ? s_cum : reinterpret_cast<const long long*>(p.cum);
-    const long long* cumt = CACHED ? s_cumt : reinterpret_cast<const long long*>(p.cumt);
-    const SetDesc* desc = CACHED ? s_desc : p.desc;
-    const long long total = done[0];
     const int n = plan_ranges(total, p.grid, p.umin);
-    auto set_of = [&](long long u) {  // last set with cum <= u
-        int lo = 0, hi = p.nsets;
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (cum[mid] <= u) lo = mid;
-            else hi = mid;
-        }
-        return lo;
-    };
     for (int w = tid; w < p.grid; w += nt) {
-        RangeRec r = {};
+        RangeRec r = {}, e = {};
         if (w < n) {
-            const long long u0 = div_small((long long)w * total, n), u1 = div_small((long long)(w + 1) * total, n);
-            r.set = set_of(u0);
-            r.d = desc[r.set];
-            const int64_t t0 = tiles_before(r.d, cum[r.set], cumt[r.set], u0, &r);
-            int64_t t1 = done[1];
+            const int64_t u0 = div_floor<int64_t>((int64_t)w * total, n), u1 = div_floor<int64_t>((int64_t)(w + 1) * total, n);
+            r.set = set_of<int64_t>(p.cum, p.nsets, u0);
+            r.d = p.desc[r.set];
+            const int64_t t0 = tiles_before<int64_t>(r.d, p.cum[r.set], p.cumt[r.set], u0, r);
+            int64_t t1 = total_t;
             if (u1 < total) {
-                const int s1 = set_of(u1);
-                t1 = tiles_before(desc[s1], cum[s1], cumt[s1], u1, nullptr);
+                const int s = set_of<int64_t>(p.cum, p.nsets, u1);
+                t1 = tiles_before<int64_t>(p.desc[s], p.cum[s], p.cumt[s], u1, e);
             }
             r.ntiles = (int)(t1 - t0);
         }
@@ -192,53 +275,30 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(PlanParams p)
     }
     if (!p.paged) return;
     for (int b = tid; b < p.rows; b += nt) {
-        RowRec r = {};
-        const SetDesc own = desc[p.ns + b];
-        r.own_u = cum[p.ns + b];
-        r.own_tiles = own.tiles;
-        if (own.own > 1) {
-            const int j = own.own - 2;
-            const SetDesc d = desc[j];
-            r.grp_u = cum[j];
-            r.grp_tiles = d.tiles;
-            r.grp_nb = d.nb;
-            r.grp_row0 = d.row0;
-            r.grp_ntok = d.ntok;
-        }
-        p.row[b] = r;
+        const SetDesc own = p.desc[p.ns + b];
+        p.row[b] = make_row(own, p.cum[p.ns + b], p.desc, own.own > 1 ? p.cum[own.own - 2] : 0);
     }
 }
 
-// the pieces of a row: of ranges w0 .. w0 + cnt - 1, first partial row base (of range 0)
-struct Pieces {
-    int w0[2], cnt[2];
-    int64_t base[2];
-};
+// ---- merge.  A row of D values is D / 4 lanes of 16 bytes, so that a workgroup has
+// 1024 / D rows of lanes.
 
-// sum over pieces first, first + step, .. of np: o, l against the running maximum m
-template <int D, typename PieceAt>
-__device__ __forceinline__ void merge_pieces(int first, int step, int np, int lane, PieceAt piece, float& m, float& l,
-                                             float (&acc)[D / 64]) {
-    constexpr int NPL = D / 64;
-    typedef float vec __attribute__((ext_vector_type(NPL == 1 ? 2 : NPL)));
+// pieces first, first + step, .. of np into o, l against their largest reference m
+template <typename PieceAt>
+__device__ __forceinline__ void merge_pieces(int first, int step, int np, int D, int lane, PieceAt piece, float& m,
+                                             float& l, f32x4& o) {
     m = -__builtin_inff();
     l = 0.0f;
-#pragma unroll
-    for (int e = 0; e < NPL; ++e) acc[e] = 0.0f;
-    constexpr int U = 8;
+    o = f32x4{0.f, 0.f, 0.f, 0.f};
+    constexpr int U = 4;
     for (int i0 = first; i0 < np; i0 += U * step) {
-        float x[U][NPL];
+        f32x4 x[U];
         float2 ml[U];
 #pragma unroll
         for (int i = 0; i < U; ++i) {
             const float* s = piece(min(i0 + i * step, np - 1));
             ml[i] = *reinterpret_cast<const float2*>(s + D);
-            if constexpr (NPL == 1) x[i][0] = s[lane];
-            else {
-                const vec y = *reinterpret_cast<const vec*>(s + NPL * lane);
-#pragma unroll
-                for (int e = 0; e < NPL; ++e) x[i][e] = y[e];
-            }
+            x[i] = *reinterpret_cast<const f32x4*>(s + 4 * lane);
         }
         float mx = m;
 #pragma unroll
@@ -247,7 +307,7 @@ __device__ __forceinline__ void merge_pieces(int first, int step, int np, int la
         m = mx;
         l = a == 0.0f ? 0.0f : l * a;
 #pragma unroll
-        for (int e = 0; e < NPL; ++e) acc[e] = a == 0.0f ? 0.0f : acc[e] * a;
+        for (int e = 0; e < 4; ++e) o[e] = a == 0.0f ? 0.0f : o[e] * a;
 #pragma unroll
         for (int i = 0; i < U; ++i) {
             // (a piece of weight 0 adds nothing, not 0 * inf; a NaN reference stays one)
@@ -255,72 +315,83 @@ __device__ __forceinline__ void merge_pieces(int first, int step, int np, int la
             const float wt = in ? __builtin_amdgcn_exp2f(ml[i].x - mx) : 0.0f;
             l = wt == 0.0f ? l : __builtin_fmaf(wt, ml[i].y, l);
 #pragma unroll
-            for (int e = 0; e < NPL; ++e) acc[e] = wt == 0.0f ? acc[e] : __builtin_fmaf(wt, x[i][e], acc[e]);
+            for (int e = 0; e < 4; ++e) o[e] = wt == 0.0f ? o[e] : __builtin_fmaf(wt, x[i][e], o[e]);
         }
     }
 }
 
-// Paged calls: one workgroup per row and query head; its waves take every fourth piece
-// of the group's common keys and of the row's own.
+template <bool BF>
+__device__ __forceinline__ u32x2 pack_row4(f32x4 o, float l) {
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    return u32x2{(uint32_t)f32_to_half<BF>(o[0] * inv) | ((uint32_t)f32_to_half<BF>(o[1] * inv) << 16),
+                 (uint32_t)f32_to_half<BF>(o[2] * inv) | ((uint32_t)f32_to_half<BF>(o[3] * inv) << 16)};
+}
+
+// Paged calls: one workgroup per row and query head, the pieces of the group's common
+// keys and of the row's own spread over its rows of lanes.
 template <int D, bool BF>
 __global__ void __launch_bounds__(256) shared_merge_paged_kernel(TileParams p, int RB) {
-    constexpr int NPL = D / 64;
-    __shared__ float so[4][D], sml[4][2];
-    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    constexpr int LR = D / 4, NG = 256 / LR;
+    __shared__ __attribute__((aligned(16))) float so[NG][D];
+    __shared__ float2 sml[NG];
+    const int lane = threadIdx.x % LR, grp = threadIdx.x / LR;
     const int b = blockIdx.x / p.Hq, hq = blockIdx.x % p.Hq, g = hq / p.G;
     const int64_t total = p.cum[p.nsets];
     const RowRec rec = p.row[b];
     const int n = plan_ranges(total, p.grid, p.umin);
-    Pieces pc = {};
+    int w0[2] = {0, 0}, cnt[2] = {0, 0};  // first range and pieces: common keys, own keys
+    int64_t base[2] = {0, 0};             // partial row of range 0
     if (rec.grp_tiles) {
         const int r = (b - rec.grp_row0) * p.G + hq % p.G, rb = r / RB;
         const int64_t u = rec.grp_u + ((int64_t)g * rec.grp_nb + rb) * (rec.grp_tiles + kItemCost) + kItemCost;
-        pc.w0[0] = plan_range_of(u, total, n);
-        pc.cnt[0] = plan_range_of(u + rec.grp_tiles - 1, total, n) - pc.w0[0] + 1;
-        pc.base[0] = plan_rows_paged(0, RB, p.Hq, p.G, p.total_rows, 0, rec.grp_row0, rec.grp_ntok, g, rb) + r % RB;
+        w0[0] = plan_range_of(u, total, n);
+        cnt[0] = plan_range_of(u + rec.grp_tiles - 1, total, n) - w0[0] + 1;
+        base[0] = plan_rows_paged(0, RB, p.Hq, p.G, p.total_rows, 0, rec.grp_row0, rec.grp_ntok, g, rb) + r % RB;
     }
     if (rec.own_tiles) {
         const int r = hq % p.G, rb = r / RB, nb = (p.G + RB - 1) / RB;
         const int64_t u = rec.own_u + ((int64_t)g * nb + rb) * (rec.own_tiles + kItemCost) + kItemCost;
-        pc.w0[1] = plan_range_of(u, total, n);
-        pc.cnt[1] = plan_range_of(u + rec.own_tiles - 1, total, n) - pc.w0[1] + 1;
-        pc.base[1] = plan_rows_paged(0, RB, p.Hq, p.G, p.total_rows, 1, b, 1, g, rb) + r % RB;
+        w0[1] = plan_range_of(u, total, n);
+        cnt[1] = plan_range_of(u + rec.own_tiles - 1, total, n) - w0[1] + 1;
+        base[1] = plan_rows_paged(0, RB, p.Hq, p.G, p.total_rows, 1, b, 1, g, rb) + r % RB;
     }
     auto piece = [&](int i) __attribute__((always_inline)) -> const float* {
-        const int k = i >= pc.cnt[0] ? 1 : 0;
-        const int at = (k ? pc.w0[1] - pc.cnt[0] : pc.w0[0]) + i;
-        return p.part + ((int64_t)at * RB + (k ? pc.base[1] : pc.base[0])) * (D + 4);
+        const int k = i >= cnt[0] ? 1 : 0;
+        const int at = (k ? w0[1] - cnt[0] : w0[0]) + i;
+        return p.part + ((int64_t)at * RB + (k ? base[1] : base[0])) * (D + 4);
     };
-    float m, l, acc[NPL];
-    merge_pieces<D>(w, 4, pc.cnt[0] + pc.cnt[1], lane, piece, m, l, acc);
-#pragma unroll
-    for (int e = 0; e < NPL; ++e) so[w][NPL * lane + e] = acc[e];
-    if (lane == 0) {
-        sml[w][0] = m;
-        sml[w][1] = l;
-    }
+    float m, l;
+    f32x4 o;
+    merge_pieces(grp, NG, cnt[0] + cnt[1], D, lane, piece, m, l, o);
+    *reinterpret_cast<f32x4*>(&so[grp][4 * lane]) = o;
+    if (lane == 0) sml[grp] = make_float2(m, l);
     __syncthreads();
-    if (threadIdx.x >= D) return;
-    float mx = sml[0][0];
+    if (threadIdx.x >= LR) return;
+    float2 x[NG];
+    float mx = -__builtin_inff(), ls = 0.0f;
 #pragma unroll
-    for (int i = 1; i < 4; ++i) mx = fmaxf(mx, sml[i][0]);
-    float o = 0.0f, ls = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float wt = sml[i][0] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(sml[i][0] - mx);
-        o = wt == 0.0f ? o : __builtin_fmaf(wt, so[i][threadIdx.x], o);
-        ls = wt == 0.0f ? ls : __builtin_fmaf(wt, sml[i][1], ls);
+    for (int i = 0; i < NG; ++i) {
+        x[i] = sml[i];
+        mx = fmaxf(mx, x[i].x);
     }
-    p.out[(int64_t)blockIdx.x * D + threadIdx.x] = f32_to_half<BF>(ls == 0.0f ? 0.0f : o / ls);
+    o = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < NG; ++i) {
+        const float wt = x[i].x == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(x[i].x - mx);
+        const f32x4 y = *reinterpret_cast<const f32x4*>(&so[i][4 * lane]);
+        ls = wt == 0.0f ? ls : __builtin_fmaf(wt, x[i].y, ls);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = wt == 0.0f ? o[e] : __builtin_fmaf(wt, y[e], o[e]);
+    }
+    *reinterpret_cast<u32x2*>(p.out + (int64_t)blockIdx.x * D + 4 * lane) = pack_row4<BF>(o, ls);
 }
 
 // Contiguous calls: workgroup (x, y) has the item that range x begins and does not
-// finish, if there is one (whole items are written already), and 16 of its
+// finish, if there is one (whole items are written already), and 1024 / D of its
 // rows; and sets without keys, whose rows are zero.
 template <int D, bool BF>
 __global__ void __launch_bounds__(256) shared_merge_local_kernel(TileParams p, int RB) {
-    constexpr int NPL = D / 64;
-    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    constexpr int LR = D / 4, NG = 256 / LR;
     const int w = blockIdx.x;
     for (int s = w; s < p.ns; s += p.grid) {
         const SetDesc d = p.desc[s];
@@ -333,24 +404,21 @@ __global__ void __launch_bounds__(256) shared_merge_local_kernel(TileParams p, i
     const RangeRec rec = p.range[w + 1], me = p.range[w];
     // the next range begins inside an item, which began here: not before this range
     if (rec.t == 0 || (me.set == rec.set && me.g == rec.g && me.rb == rec.rb && me.t > 0)) return;
-    const int nrow = min(RB, rec.d.ntok * p.G - RB * rec.rb), r0 = 16 * blockIdx.y + 4 * wv;
-    if (r0 >= nrow) return;
+    const int lane = threadIdx.x % LR, r = NG * blockIdx.y + threadIdx.x / LR;
+    if (r >= min(RB, rec.d.ntok * p.G - RB * rec.rb)) return;
     const int64_t total = p.cum[p.nsets];
     const int n = plan_ranges(total, p.grid, p.umin);
     const int64_t last = p.cum[rec.set] + ((int64_t)rec.g * rec.d.nb + rec.rb + 1) * (rec.d.tiles + kItemCost) - 1;
     const int cnt = plan_range_of(last, total, n) - w + 1;
-    for (int r = r0; r < min(r0 + 4, nrow); ++r) {
-        auto piece = [&](int i) __attribute__((always_inline)) -> const float* {
-            return p.part + (plan_rows_local(w + i, RB, i > 0) + r) * (D + 4);
-        };
-        float m, l, acc[NPL];
-        merge_pieces<D>(0, 1, cnt, lane, piece, m, l, acc);
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        const int x = RB * rec.rb + r;
-        uint16_t* op = p.out + ((rec.d.row0 + x / p.G) * (int64_t)p.Hq + rec.g * p.G + x % p.G) * D + NPL * lane;
-#pragma unroll
-        for (int e = 0; e < NPL; ++e) op[e] = f32_to_half<BF>(acc[e] * inv);
-    }
+    auto piece = [&](int i) __attribute__((always_inline)) -> const float* {
+        return p.part + (plan_rows_local(w + i, RB, i > 0) + r) * (D + 4);
+    };
+    float m, l;
+    f32x4 o;
+    merge_pieces(0, 1, cnt, D, lane, piece, m, l, o);
+    const int x = RB * rec.rb + r;
+    *reinterpret_cast<u32x2*>(p.out + ((rec.d.row0 + x / p.G) * (int64_t)p.Hq + rec.g * p.G + x % p.G) * D + 4 * lane) =
+        pack_row4<BF>(o, l);
 }
 
 template <int D, bool BF>
@@ -360,7 +428,7 @@ void launch_merge_d(const TileParams& p, int RB, hipStream_t s) {
         hipLaunchKernelGGL((shared_merge_paged_kernel<D, BF>), dim3((unsigned)rows), dim3(256), 0, s, p, RB);
         return;
     }
-    hipLaunchKernelGGL((shared_merge_local_kernel<D, BF>), dim3((unsigned)p.grid, (unsigned)RB / 16), dim3(256), 0, s, p,
+    hipLaunchKernelGGL((shared_merge_local_kernel<D, BF>), dim3((unsigned)p.grid, (unsigned)(RB * D / 1024)), dim3(256), 0, s, p,
                        RB);
 }
 
@@ -451,9 +519,14 @@ int shared_tiles(const SharedArgs& a, void* ws, hipStream_t s) {
     pl.grid = sh.grid;
     pl.umin = kUnitsMin;
     pl.gs = reinterpret_cast<int32_t*>(w + sh.gs);
-    const int threads = pl.nsets > 512 || sh.grid > 512 ? kPlanThreads : 512;
-    if (pl.nsets <= kPlanCached) hipLaunchKernelGGL(shared_plan_kernel<true>, dim3(1), dim3(threads), 0, s, pl);
-    else hipLaunchKernelGGL(shared_plan_kernel<false>, dim3(1), dim3(threads), 0, s, pl);
+    // units fit 32 bits where even the longest sets that fit the call do
+    const int64_t tiles = paged ? pl.max_keys / 64 + 2 : a.num_keys / 64 + 2;
+    const int64_t items = (int64_t)a.Hkv * (((int64_t)a.rows * pl.G / kTileRows + a.nsets) + (paged ? (int64_t)a.rows * ((pl.G - 1) / kTileRows + 1) : 0));
+    const int need = std::max({pl.nsets, a.nsets + 1, sh.whole ? 1 : sh.grid + 1});
+    if (need <= kPlanCached && items < 0x7fffffff / (tiles + kItemCost))
+        hipLaunchKernelGGL(shared_plan_kernel, dim3(1), dim3((unsigned)(need + 63) / 64 * 64), 0, s, pl);
+    else
+        hipLaunchKernelGGL(shared_plan_long_kernel, dim3(1), dim3(kPlanThreads), 0, s, pl);
     VMC_LAUNCH_CHECK();
 
     TileParams p = {};
