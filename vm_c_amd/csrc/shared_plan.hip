@@ -452,8 +452,7 @@ struct Shape {
 Shape shape_of(bool paged, int rows, int nsets, int Hq, int Hkv, int D) {
     Shape sh = {};
     const int64_t G = Hq / Hkv, sets = std::max(nsets, 1);
-    // workgroups that fit a CU: 64 KB of tiles each (head_dim 256: 128 KB)
-    sh.grid = num_cus() * (D == 256 ? 1 : 2);
+    sh.grid = num_cus() * tile_per_cu(D);
     // Whole items where sets of many rows give several times the workgroups
     const int64_t items = (int64_t)Hkv * (rows * G / kTileRows + std::min<int64_t>(rows, sets));
     if (!paged && rows * G >= kTileRows * sets && items >= 4 * (int64_t)sh.grid && items < (1 << 30)) {

@@ -125,7 +125,7 @@ __device__ __noinline__ void shared_row_exact(const uint16_t* q, const uint8_t* 
 // BF: the products' type (LOCAL and PAGED: the rows'; GGUF: fp16, BF false);
 // QBF: the type of q and out
 template <int D, int SRC, bool QBF, bool CONV>
-__global__ void __launch_bounds__(256, D == 256 ? 1 : 2) shared_tile_kernel(TileParams p) {
+__global__ void __launch_bounds__(256, tile_per_cu(D)) shared_tile_kernel(TileParams p) {
     constexpr int W = kTileWaves;
     constexpr bool kGguf = SRC == TS_Q8 || SRC == TS_Q4;
     constexpr bool BF = QBF && !kGguf;
@@ -193,12 +193,14 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) shared_tile_kernel(Tile
     };
     Cursor cc;  // of the tile in use
     int range = blockIdx.x, units;
+    SetDesc first;
     if (arg()->whole) {  // one item; consecutive items to one XCD, whose L2 holds their keys
         const int64_t total = as_const(p.cum)[p.nsets], per = (total + 7) >> 3;
         const int64_t item = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
         if ((blockIdx.x >> 3) >= per || item >= total) return;
         cc.set = plan_find(p.cum, p.nsets, item, lane);
-        take(cc, desc_of(cc.set));
+        first = desc_of(cc.set);
+        take(cc, first);
         const int in_set = (int)(item - as_const(p.cum)[cc.set]);
         cc.t = 0;
         cc.g = in_set / cc.nb;
@@ -211,7 +213,8 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) shared_tile_kernel(Tile
         cc.rb = r[2];
         cc.t = r[3];
         units = r[4];
-        take(cc, SetDesc{r[8], r[9], r[10], r[11], r[12], r[13], r[14], r[15]});
+        first = SetDesc{r[8], r[9], r[10], r[11], r[12], r[13], r[14], r[15]};
+        take(cc, first);
         if (units == 0) return;
     }
     units = __builtin_amdgcn_readfirstlane(units);
@@ -441,9 +444,8 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) shared_tile_kernel(Tile
     int lo = 0, hi = 0, hi_min = 0;  // keys of this lane's row, the least end of the wave's rows
     bool active = false;             // the wave has rows of the item
 
-    auto begin_item = [&]() __attribute__((always_inline)) {  // cc's
+    auto begin_item = [&](const SetDesc& d) __attribute__((always_inline)) {  // cc's, of set d
         const auto* a = arg();
-        const SetDesc d = desc_of(cc.set);
         const int G = a->G, nrow = min(RB, d.ntok * G - RB * cc.rb);
         active = 32 * w < nrow;
         if (!active) return;
@@ -759,6 +761,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) shared_tile_kernel(Tile
     fetch();
     load(0);
     if (!kGguf && NS == 3 && loaded < units) load(1);
+    begin_item(first);  // (its reads overlap the first tile's)
     if constexpr (kConv) {
         landed(0);
         convert(0, 0);
@@ -768,7 +771,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) shared_tile_kernel(Tile
         if constexpr (kGguf) stage(slot);
         else if constexpr (!kConv) landed(u);
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (u == 0 || cc.t == 0) begin_item();
+        if (u > 0 && cc.t == 0) begin_item(desc_of(cc.set));
         const uint32_t valid = (vq >> (4 * (fetched - 1 - u))) & 15u;
         if (loaded < units) load(fill);
         f32x4 vexp = {0.0f, 0.0f, 0.0f, 0.0f};
