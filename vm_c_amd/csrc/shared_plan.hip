@@ -507,7 +507,7 @@ int shared_tiles(const SharedArgs& a, void* ws, hipStream_t s) {
     pl.num_keys = a.num_keys;
     pl.Hkv = a.Hkv;
     pl.G = a.Hq / a.Hkv;
-    pl.RB = kTileRows;
+    pl.RB = a.src == GEN_Q8 || a.src == GEN_Q4 ? kTileRows / 2 : kTileRows;
     pl.paged = paged;
     pl.whole = sh.whole;
     pl.cum = reinterpret_cast<int64_t*>(w + sh.cum);
@@ -520,7 +520,7 @@ int shared_tiles(const SharedArgs& a, void* ws, hipStream_t s) {
     pl.gs = reinterpret_cast<int32_t*>(w + sh.gs);
     // units fit 32 bits where even the longest sets that fit the call do
     const int64_t tiles = paged ? pl.max_keys / 64 + 2 : a.num_keys / 64 + 2;
-    const int64_t items = (int64_t)a.Hkv * (((int64_t)a.rows * pl.G / kTileRows + a.nsets) + (paged ? (int64_t)a.rows * ((pl.G - 1) / kTileRows + 1) : 0));
+    const int64_t items = (int64_t)a.Hkv * (((int64_t)a.rows * pl.G / pl.RB + a.nsets) + (paged ? (int64_t)a.rows * ((pl.G - 1) / pl.RB + 1) : 0));
     const int need = std::max({pl.nsets, a.nsets + 1, sh.whole ? 1 : sh.grid + 1});
     if (need <= kPlanCached && items < 0x7fffffff / (tiles + kItemCost))
         hipLaunchKernelGGL(shared_plan_kernel, dim3(1), dim3((unsigned)(need + 63) / 64 * 64), 0, s, pl);

@@ -43,7 +43,7 @@ struct RowRec {
 constexpr int kItemCost = 2;
 
 constexpr int kTileWaves = 4;  // waves of the shared-keys kernel, 32 rows each
-constexpr int kTileRows = 32 * kTileWaves;  // rows of an item
+constexpr int kTileRows = 32 * kTileWaves;  // rows of an item (GGUF pages: half)
 // its workgroups that fit a CU: 64 KB of tiles (head_dim 64: 48, 256: 128), 168 registers a
 // lane at head_dim 64, 256 at 128, 512 at 256
 __host__ __device__ constexpr int tile_per_cu(int D) { return D == 64 ? 3 : D == 128 ? 2 : 1; }

@@ -20,10 +20,10 @@
 //   operands come from the row-major tile by transposing LDS reads, and the
 //   contraction index is permuted as P leaves the S registers (k = 8h + e <->
 //   key 16c + 8 (e / 4) + 4h + e % 4).
-//   A wave has 32 of the block's rows; waves beyond the rows only load.
+//   A wave has 32 of the item's rows; waves beyond the rows only load.
 // 16-bit rows arrive by load-to-LDS transfers, two or three tile slots; GGUF
 // blocks through registers, dequantized to fp16 (code * d rounded once: 2^-11
-// of a value at most).
+// of a value at most) by two waves for the two that have rows.
 //
 // Weights enter P . V as fp16 where that costs nothing the result shows: half a step is
 // 2^-11 of a weight, beside the 2^-8 of a bf16 result.  bf16 V becomes fp16 for
@@ -134,15 +134,17 @@ __global__ void __launch_bounds__(256, tile_per_cu(D)) shared_tile_kernel(TilePa
     constexpr int ROW = 2 * D, TILE = kBN * ROW;
     constexpr int NS = kGguf || D != 64 ? 2 : 3;      // slots
     constexpr int NTR = TILE / (1024 * W);            // transfers per wave and tensor
-    constexpr int RB = 32 * W;                        // rows of an item
+    constexpr int CW = kGguf ? W / 2 : W;             // waves with rows; the others dequantize
+    constexpr int RB = 32 * CW;                       // rows of an item
     constexpr bool kConv = CONV;                      // bf16 V is converted to fp16
     static_assert(!CONV || BF, "fp16 V needs no conversion");
     constexpr bool PBF = BF && !kConv;                // the type of P . V
     constexpr int NT = PBF || !QBF ? 2 : 1;           // terms of a weight
     constexpr float kOff = PBF ? 0.0f : 7.0f;         // weights are 2^(s - m + kOff), at most 2^15
     constexpr int HB = D == 256 ? 1 : 2;              // 32-key blocks per softmax round
-    // GGUF: blocks per lane and tile (K's then V's), dwords from a block's 4-byte floor
-    constexpr int NBL = D / (16 * W) > 0 ? D / (16 * W) : 1;
+    // GGUF: blocks per dequantizing lane and tile (K's then V's), dwords from a block's
+    // 4-byte floor
+    constexpr int LOADERS = 64 * (W - CW), NBL = kGguf ? 4 * D / (kGguf ? LOADERS : 1) : 1;
     constexpr int BE = SRC == TS_Q8 ? 34 : 18, NWD = SRC == TS_Q8 ? 9 : 5;
     struct Lds {
         uint8_t tile[NS][2][TILE];                       // [slot][K, V]
@@ -324,10 +326,9 @@ __global__ void __launch_bounds__(256, tile_per_cu(D)) shared_tile_kernel(TilePa
         if constexpr (kGguf) {
 #pragma unroll
             for (int i = 0; i < NBL; ++i) {
-                const int idx = i * 64 * W + tid;
+                const int idx = i * LOADERS + tid - 64 * CW;
                 const bool is_v = idx >= 2 * D;
                 const int x = idx & (2 * D - 1), r = x / (D / 32), blk = x % (D / 32), c = r >> 4;
-                if (NBL * 64 * W > 4 * D && idx >= 4 * D) continue;
                 int64_t off = rec.k[0];
 #pragma unroll
                 for (int e = 1; e < NA; ++e) off = c == e ? rec.k[e] : off;
@@ -351,10 +352,9 @@ __global__ void __launch_bounds__(256, tile_per_cu(D)) shared_tile_kernel(TilePa
         if constexpr (kGguf) {
 #pragma unroll
             for (int i = 0; i < NBL; ++i) {
-                const int idx = i * 64 * W + tid;
+                const int idx = i * LOADERS + tid - 64 * CW;
                 const bool is_v = idx >= 2 * D;
                 const int x = idx & (2 * D - 1), r = x / (D / 32), blk = x % (D / 32);
-                if (NBL * 64 * W > 4 * D && idx >= 4 * D) continue;
                 const bool odd = (blk & 1) != 0;
                 uint32_t c[NWD - 1];
 #pragma unroll
@@ -447,7 +447,7 @@ __global__ void __launch_bounds__(256, tile_per_cu(D)) shared_tile_kernel(TilePa
     auto begin_item = [&](const SetDesc& d) __attribute__((always_inline)) {  // cc's, of set d
         const auto* a = arg();
         const int G = a->G, nrow = min(RB, d.ntok * G - RB * cc.rb);
-        active = 32 * w < nrow;
+        active = w < CW && 32 * w < nrow;
         if (!active) return;
         const int r = RB * cc.rb + min(32 * w + c32, nrow - 1);
         const int64_t tok = d.row0 + r / G;
@@ -741,7 +741,7 @@ __global__ void __launch_bounds__(256, tile_per_cu(D)) shared_tile_kernel(TilePa
     int loaded = 0, seg_t0 = cc.t;
     auto load = [&](uint32_t slot) __attribute__((always_inline)) {  // the record's tile
         if constexpr (kGguf) {
-            load_blocks();
+            load_blocks();  // into registers
         } else {
             transfer(false, rec, lds0 + slot * (2u * TILE));
             transfer(true, rec, lds0 + slot * (2u * TILE) + TILE);
@@ -755,38 +755,70 @@ __global__ void __launch_bounds__(256, tile_per_cu(D)) shared_tile_kernel(TilePa
             else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         }
     };
-    // Tile u in slot u % NS, the next NS - 1 in flight while it runs (GGUF: the next in
-    // registers).  The barrier makes tile u visible and shows slot (u - 1) % NS
-    // free, which then receives tile u + NS - 1.
-    fetch();
-    load(0);
-    if (!kGguf && NS == 3 && loaded < units) load(1);
-    begin_item(first);  // (its reads overlap the first tile's)
-    if constexpr (kConv) {
-        landed(0);
-        convert(0, 0);
-    }
-    uint32_t slot = 0, fill = NS - 1;
-    for (int u = 0; u < units; ++u) {
-        if constexpr (kGguf) stage(slot);
-        else if constexpr (!kConv) landed(u);
-        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (u > 0 && cc.t == 0) begin_item(desc_of(cc.set));
+    auto meet = [&]() __attribute__((always_inline)) { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+    // tile u by the waves that have rows
+    auto use = [&](int u, uint32_t slot) __attribute__((always_inline)) {
         const uint32_t valid = (vq >> (4 * (fetched - 1 - u))) & 15u;
-        if (loaded < units) load(fill);
         f32x4 vexp = {0.0f, 0.0f, 0.0f, 0.0f};
         if constexpr (kConv) vexp = *reinterpret_cast<const f32x4*>(lds.vexp[u & 1]);
         if (active) process(slot, valid, vexp);
-        const bool more = u + 1 < units, ends = cc.t + 1 == cc.tiles || !more;
+        const bool ends = cc.t + 1 == cc.tiles || u + 1 == units;
         if (ends && active) end_item(cc.set, cc.g, cc.rb, seg_t0, cc.t + 1);
-        slot = slot == NS - 1 ? 0 : slot + 1;
-        fill = fill == NS - 1 ? 0 : fill + 1;
-        if (more) {
+        if (u + 1 < units) {
             advance(cc);
             if (ends) seg_t0 = cc.t;
+        }
+    };
+    fetch();
+    if constexpr (kGguf) {
+        // Half the waves dequantize tile u + 1, and have tile u + 2 in flight, while the others
+        // use tile u: one after the other in each wave, the two took 2.8 us a tile, with
+        // few rows and with many (head_dim 128)
+        if (w >= CW) {
+            load(0);
+            stage(0);
+            if (loaded < units) load(0);
+            meet();
+            for (int u = 0; u < units; ++u) {
+                if (u + 1 < units) stage((u + 1) & 1);
+                if (loaded < units) load(0);
+                meet();
+            }
+        } else {
+            fetch();
+            begin_item(first);
+            meet();
+            for (int u = 0; u < units; ++u) {
+                if (u > 0 && cc.t == 0) begin_item(desc_of(cc.set));
+                use(u, u & 1);
+                fetch();
+                meet();
+            }
+        }
+    } else {
+        // Tile u in slot u % NS, the next NS - 1 in flight while it runs.  The barrier makes tile
+        // u visible and shows slot (u - 1) % NS free, which then receives tile u + NS - 1.
+        load(0);
+        if (NS == 3 && loaded < units) load(1);
+        begin_item(first);  // (its reads overlap the first tile's)
+        if constexpr (kConv) {
+            landed(0);
+            convert(0, 0);
+        }
+        uint32_t slot = 0, fill = NS - 1;
+        for (int u = 0; u < units; ++u) {
+            if constexpr (!kConv) landed(u);
+            meet();
+            if (u > 0 && cc.t == 0) begin_item(desc_of(cc.set));
+            if (loaded < units) load(fill);
+            use(u, slot);
+            slot = slot == NS - 1 ? 0 : slot + 1;
+            fill = fill == NS - 1 ? 0 : fill + 1;
             if constexpr (kConv) {
-                landed(u + 1);
-                convert(slot, (u + 1) & 1);
+                if (u + 1 < units) {
+                    landed(u + 1);
+                    convert(slot, (u + 1) & 1);
+                }
             }
         }
     }
