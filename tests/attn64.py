@@ -34,21 +34,25 @@ def attend(q, k, v, scale, qt, e_k=0.0, e_v=0.0, mixed=False):
     # roundings in sequence
     n_seq = 64 + 3 * (len(k) // 64 + 1) / 16
     es = n_seq * 2.0 ** -24
-    # weights on their way into the products with V (the sum of the weights takes them
-    # unrounded): for a bf16 result one fp16 term, half a step of which is 2^-11; for
-    # an fp16 result two terms, of which a first bf16 one leaves 2^-8 and a second
+    # weights on their way into the products with V.  For a bf16 result one fp16 term,
+    # cut: off by x_k in 0 .. 2^-10, in the sum of the weights too, so that
+    # o moves by sum_k w_k x_k (v_k - o), where any constant may be taken off x
+    # (sum_k w_k (v_k - o) = 0): 2^-11 sum_k w_k |v_k - o| at most.  For
+    # an fp16 result (a bf16 one of few rows is no worse) two terms, and a sum of the
+    # weights as they were: a first bf16 term leaves 2^-8 and a second
     # half a step of its own binade, 2^-17 of the weight
     ew = 2.0 ** -11 if qt == "bf16" else 2.0 ** -17
     av = w @ np.abs(v)
     err = (w * ds) @ (np.abs(v) + np.abs(o)) + es * (av + np.abs(o)) + (ew + e_v) * av
-    # bf16 V as fp16, 16 keys by a power of two: off by 2^-25 over the scale, which is 2^8,
-    # or 1 beside values of 256 and more.  Weights of 2^-32 of the largest and less meet
+    # bf16 V as fp16, 16 keys by a power of two: cut, off by 2^-24 over the scale, which is 2^8,
+    # or 1 beside values of 256 and more.  Weights of 2^-31 of the largest and less meet
     # the end of fp16, 2^20 earlier where a chunk is scaled that much more than another
     if qt == "bf16":
-        err = err + 2.0 ** (-25 if mixed else -33)
+        err = err + ew * np.abs(o) + 2.0 ** -31 * w.max() * (np.abs(v).sum(0) + len(v) * np.abs(o))
+        err = err + 2.0 ** (-24 if mixed else -32)
         if mixed:
-            err = err + 2.0 ** -12 * w.max() * np.abs(v * (np.abs(v).max(1, keepdims=True) < 2.0 ** -12)).sum(0)
-            err = err + 2.0 ** -24 * w.max() * np.abs(v).sum(0)
+            err = err + 2.0 ** -11 * w.max() * np.abs(v * (np.abs(v).max(1, keepdims=True) < 2.0 ** -12)).sum(0)
+            err = err + 2.0 ** -23 * w.max() * np.abs(v).sum(0)
     err = err * 1.02  # second order
     return o, err + (np.abs(o) + err) * HALF_STEP[qt] + TINY[qt]
 

@@ -25,13 +25,14 @@
 // blocks through registers, dequantized to fp16 (code * d rounded once: 2^-11
 // of a value at most) by two waves for the two that have rows.
 //
-// Weights enter P . V as fp16 where that costs nothing the result shows: half a step is
-// 2^-11 of a weight, beside the 2^-8 of a bf16 result.  bf16 V becomes fp16 for
-// it, by the waves that fetched its rows, while slower waves still multiply:
+// Weights enter P . V as fp16 where that costs nothing the result shows: two of them cut
+// to fp16 by one instruction, and summed as they were cut by another, so that the cut
+// (0 to 2^-10 of a weight) stays out of their mean, and 2^-11 of a value at most is
+// left, beside the 2^-8 of a bf16 result.  bf16 V becomes fp16 for it, by the waves that fetched its rows, while slower waves still multiply:
 // each 16 keys times 2^8 (values up to 255), 1 (larger ones) or 2^20 (all below
 // 2^-12), which their weights undo against the largest of an item's.  So values from
-// 2^-33 to 65504 keep their bits; the smaller ones of a chunk are off by 2^-25 over
-// its scale at most.  A chunk outside that range
+// 2^-33 to 65504 keep their bits; the smaller ones of a chunk are cut, off by 2^-24
+// over its scale at most.  A chunk outside that range
 // makes its rows rerun.  Elsewhere (fp16 results; few rows, where the products
 // are not what counts) weights are two 16-bit terms of V's type, which leave
 // 2^-17 (bf16) or 2^-23 (fp16) of a weight: one term of 8 bits, or of the result's
@@ -400,16 +401,17 @@ __global__ void __launch_bounds__(256, tile_per_cu(D)) shared_tile_kernel(TilePa
             const bool big = __ballot(m >= 0x4380u) != 0, tiny = __ballot(m >= 0x3980u) == 0;
             // past 65504 (or no number), or all below 2^-33 but not 0: no scale fits
             const bool bad = __ballot(m >= 0x4780u) != 0 || (__ballot(m >= 0x2f00u) == 0 && __ballot(m != 0) != 0);
-            const float scale = big ? 1.0f : tiny ? 1048576.0f : 256.0f;
+            // (added to the exponents; a 0 becomes a number below fp16's, cut to 0 again)
+            const uint32_t up = big ? 0u : tiny ? 20u << 23 : 8u << 23;
             if (lane == 0) lds.vexp[half][w] = bad ? __builtin_nanf("") : big ? 8.0f : tiny ? -12.0f : 0.0f;
 #pragma unroll
             for (int i = 0; i < NTR; ++i) {
                 u32x4 y;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float f0 = bf16_bits_to_f32((uint16_t)(x[i][e] & 0xffffu)) * scale;
-                    const float f1 = bf16_bits_to_f32((uint16_t)(x[i][e] >> 16)) * scale;
-                    y[e] = (uint32_t)f32_to_f16_bits(f0) | ((uint32_t)f32_to_f16_bits(f1) << 16);
+                    const uint32_t f0 = (x[i][e] << 16) + up, f1 = (x[i][e] & 0xffff0000u) + up;
+                    y[e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(__builtin_bit_cast(float, f0),
+                                                                                   __builtin_bit_cast(float, f1)));
                 }
                 *reinterpret_cast<u32x4*>(at + 1024 * i) = y;
             }
@@ -593,10 +595,12 @@ __global__ void __launch_bounds__(256, tile_per_cu(D)) shared_tile_kernel(TilePa
                     const int j = 4 * (2 * (c & 1) + (e >> 2)) + (e & 3);
                     const float x0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[c >> 1][j], csc, off));
                     const float x1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[c >> 1][j + 1], csc, off));
-                    part += x0 + x1;
                     if constexpr (NT == 1) {
-                        pt[0][c][e >> 1] = (uint32_t)f32_to_half<PBF>(x0) | ((uint32_t)f32_to_half<PBF>(x1) << 16);
+                        const auto xh = __builtin_amdgcn_cvt_pkrtz(x0, x1);
+                        part = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, xh), f16x2{1, 1}, part, false);
+                        pt[0][c][e >> 1] = __builtin_bit_cast(uint32_t, xh);
                     } else {
+                        part += x0 + x1;
                         uint32_t t0, t1;
                         two_terms<PBF>(x0, x1, t0, t1);
                         pt[0][c][e >> 1] = t0;
