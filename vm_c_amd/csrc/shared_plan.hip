@@ -4,7 +4,7 @@
 // The plan is one workgroup's: lengths and starts live on the device, so a captured
 // call follows them, and the kernels behind it find any unit of the axis by one or
 // two rounds of 64 probes instead of scanning the batch each.
-#include "shared_plan.hpp"
+#include "shared_plan_dev.hpp"
 
 #include <algorithm>
 
@@ -15,201 +15,29 @@ namespace vmc {
 namespace {
 
 constexpr int kPlanThreads = 1024;
-constexpr int kUnitsMin = kItemCost + 1;  // fewest units of a range: one tile
 constexpr int kPlanCached = 1024;         // sets, and ranges, that the short plan holds in LDS
-
-// Inclusive scan over the wave in six DPP steps (row_shr 1, 2, 4, 8, then the last lane of
-// the row before, then lane 31); op(v, 0) = v for the values scanned
-template <typename Op>
-__device__ __forceinline__ int wave_scan(int v, Op op) {
-    v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true));
-    v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true));
-    v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true));
-    v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true));
-    v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false));
-    v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false));
-    return v;
-}
-// over the workgroup (16 waves at most; sh: 16 entries); all: the last one's
-template <typename Op>
-__device__ __forceinline__ int block_scan(int v, int* sh, Op op, int& all) {
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, nw = blockDim.x >> 6;
-    v = wave_scan(v, op);
-    if (lane == 63) sh[w] = v;
-    __syncthreads();
-    int x[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] = sh[i];
-    int run = 0, before = 0;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        before = i < w ? op(run, x[i]) : before;
-        run = i < nw ? op(run, x[i]) : run;
-    }
-    all = run;
-    __syncthreads();
-    return op(v, before);
-}
-__device__ __forceinline__ long long block_scan(long long v, long long* sh, long long& all) {
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, nw = blockDim.x >> 6;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const long long o = __shfl_up(v, d, kWave);
-        if (lane >= d) v += o;
-    }
-    if (lane == 63) sh[w] = v;
-    __syncthreads();
-    long long before = 0;
-    all = 0;
-    for (int i = 0; i < nw; ++i) {
-        before += i < w ? sh[i] : 0;
-        all += sh[i];
-    }
-    __syncthreads();
-    return v + before;
-}
-
-template <typename T>
-__device__ __forceinline__ T div_floor(T x, T y) {  // x >= 0, y > 0
-    if constexpr (sizeof(T) == 4) return (T)((uint32_t)x / (uint32_t)y);
-    else return ((x | y) >> 32) == 0 ? (T)((uint32_t)x / (uint32_t)y) : x / y;
-}
-
-// One set, from its length (group: shared tokens; sequence: states; row: tokens)
-__device__ __forceinline__ SetDesc make_desc(const PlanParams& p, int i, int row0, int ntok, int len, int key0, int group,
-                                             int shared) {
-    SetDesc d = {};
-    if (i < p.ns) {
-        d.row0 = row0;
-        d.ntok = ntok;
-        const int n = max(len, 0);
-        if (p.paged) {
-            d.src = row0;
-            // a group of one row has nothing to share: all its keys are the row's own
-            d.khi = ntok > 1 ? min(n, p.max_keys) : 0;
-        } else {
-            const long long end = min((long long)key0 + n, (long long)p.num_keys);
-            d.src = max(key0, 0);
-            d.khi = (int)max(end - d.src, 0ll);
-        }
-    } else {
-        d.row0 = d.src = i - p.ns;
-        d.ntok = 1;
-        d.khi = min(len, p.max_keys);
-        d.klo = max(shared, 0);
-        d.own = group + 2;  // 1: of no group
-    }
-    d.nb = (int)div_floor<long long>((long long)d.ntok * p.G + p.RB - 1, p.RB);
-    d.tiles = d.ntok > 0 && d.khi > d.klo ? (int)(((long long)d.khi - (d.klo & ~15) + 63) / 64) : 0;
-    return d;
-}
-// the group of a row that shares something with others, or -1: starts gs[0 .. ns]
-__device__ __forceinline__ int group_of(const int* gs, int ns, int row) {
-    int lo = 0, hi = ns + 1;  // starts that are <= row
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (gs[mid] <= row) lo = mid + 1;
-        else hi = mid;
-    }
-    return lo >= 1 && lo <= ns && gs[lo] - gs[lo - 1] > 1 ? lo - 1 : -1;
-}
-// tiles before unit u of a set (and the first tile's place at or after u)
-template <typename T>
-__device__ __forceinline__ T tiles_before(const SetDesc& d, T cum, T cumt, T u, RangeRec& rec) {
-    const T rem = u - cum, per = d.tiles + kItemCost, item = div_floor<T>(rem, per);
-    rec.t = max((int)(rem - item * per) - kItemCost, 0);
-    rec.g = (int)div_floor<T>(item, d.nb);
-    rec.rb = (int)(item - (T)rec.g * d.nb);
-    return cumt + item * d.tiles + rec.t;
-}
-// last set of n with cum <= u
-template <typename T>
-__device__ __forceinline__ int set_of(const T* cum, int n, T u) {
-    int lo = 0, hi = n;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (cum[mid] <= u) lo = mid;
-        else hi = mid;
-    }
-    return lo;
-}
-__device__ __forceinline__ RowRec make_row(const SetDesc& own, int64_t own_u, const SetDesc* desc, int64_t grp_u) {
-    RowRec r = {};
-    r.own_u = own_u;
-    r.own_tiles = own.tiles;
-    if (own.own > 1) {
-        const SetDesc d = desc[own.own - 2];
-        r.grp_u = grp_u;
-        r.grp_tiles = d.tiles;
-        r.grp_nb = d.nb;
-        r.grp_row0 = d.row0;
-        r.grp_ntok = d.ntok;
-    }
-    return r;
-}
 
 // The plan of a call of at most kPlanCached sets and ranges whose units fit 32 bits, a
 // thread a set: every step from registers and LDS.  What bounds it: its chain of
 // dependent steps.
 __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(PlanParams p) {
-    __shared__ int sh[3][16];
-    __shared__ int s_gs[kPlanCached + 1], s_len[kPlanCached], s_cum[kPlanCached + 1], s_cumt[kPlanCached + 1];
+    __shared__ PlanLds<kPlanCached, kPlanThreads / 64> lds;
     __shared__ int s_first[kPlanCached + 1];  // tiles before each range
     __shared__ SetDesc s_desc[kPlanCached];
     const int i = threadIdx.x;
-    int len = 0, key0 = 0;
-    if (i < p.ns) {
-        len = p.set_lens[i];
-        if (!p.paged) key0 = p.key_starts[i];
-    } else if (i < p.nsets) {
-        len = p.seq_lens[i - p.ns];
-    }
-    int all;
-    const int start = p.ns > 0 && i <= p.ns ? min(max(p.starts[i], 0), p.rows) : 0;
-    const int gs = block_scan(start, sh[0], [](int a, int b) { return max(a, b); }, all);
-    if (i <= p.ns) {
-        s_gs[i] = gs;
-        p.gs[i] = gs;
-    }
-    if (i < p.nsets) s_len[i] = len;
-    __syncthreads();
-    SetDesc d = {};
-    int units = 0, tiles = 0;
-    if (i < p.nsets) {
-        const int j = i < p.ns ? -1 : group_of(s_gs, p.ns, i - p.ns);
-        d = make_desc(p, i, i < p.ns ? s_gs[i] : 0, i < p.ns ? s_gs[i + 1] - s_gs[i] : 0, len, key0, j, j >= 0 ? s_len[j] : 0);
-        const int items = p.Hkv * d.nb;
-        units = p.whole ? items : d.tiles ? items * (d.tiles + kItemCost) : 0;
-        tiles = items * d.tiles;
-        p.desc[i] = d;
-        s_desc[i] = d;
-    }
-    int total, total_t;
-    const int cum = block_scan(units, sh[1], [](int a, int b) { return a + b; }, total) - units;
-    const int cumt = block_scan(tiles, sh[2], [](int a, int b) { return a + b; }, total_t) - tiles;
-    if (i < p.nsets) {
-        p.cum[i] = cum;
-        s_cum[i] = cum;
-        s_cumt[i] = cumt;
-    }
-    if (i == 0) p.cum[p.nsets] = total;
+    const PlanSums x = plan_sets(p, lds, s_desc, i);
+    plan_out(p, x, s_desc, lds.cum, i);
     if (p.whole) return;
-    __syncthreads();
-    const int n = plan_ranges(total, p.grid, p.umin);
+    const int n = plan_ranges(x.total, p.grid, p.umin);
     RangeRec r = {};
     if (i < n) {
-        const int u = (int)div_floor<long long>((long long)i * total, n);
-        r.set = set_of(s_cum, p.nsets, u);
-        r.d = s_desc[r.set];
-        r.ntiles = tiles_before(r.d, s_cum[r.set], s_cumt[r.set], u, r);
+        r.ntiles = range_begin(lds, s_desc, p.nsets, (int)div_floor<long long>((long long)i * x.total, n), r);
         s_first[i] = r.ntiles;
     }
-    if (i == 0) s_first[n] = total_t;
+    if (i == 0) s_first[n] = x.total_t;
     __syncthreads();
     if (i < n) r.ntiles = s_first[i + 1] - r.ntiles;
     if (i < p.grid) p.range[i] = r;
-    if (p.paged && i >= p.ns && i < p.nsets)
-        p.row[i - p.ns] = make_row(d, cum, s_desc, d.own > 1 ? s_cum[d.own - 2] : 0);
 }
 
 // The plan of any other call, through memory
@@ -521,14 +349,20 @@ int shared_tiles(const SharedArgs& a, void* ws, hipStream_t s) {
     // units fit 32 bits where even the longest sets that fit the call do
     const int64_t tiles = paged ? pl.max_keys / 64 + 2 : a.num_keys / 64 + 2;
     const int64_t items = (int64_t)a.Hkv * (((int64_t)a.rows * pl.G / pl.RB + a.nsets) + (paged ? (int64_t)a.rows * ((pl.G - 1) / pl.RB + 1) : 0));
+    const bool short_units = items < 0x7fffffff / (tiles + kItemCost);
     const int need = std::max({pl.nsets, a.nsets + 1, sh.whole ? 1 : sh.grid + 1});
-    if (need <= kPlanCached && items < 0x7fffffff / (tiles + kItemCost))
-        hipLaunchKernelGGL(shared_plan_kernel, dim3(1), dim3((unsigned)(need + 63) / 64 * 64), 0, s, pl);
-    else
-        hipLaunchKernelGGL(shared_plan_long_kernel, dim3(1), dim3(kPlanThreads), 0, s, pl);
-    VMC_LAUNCH_CHECK();
+    const bool fused = short_units && !sh.whole && std::max(pl.nsets, a.nsets + 1) <= kPlanFused;
+    if (!fused) {
+        if (short_units && need <= kPlanCached)
+            hipLaunchKernelGGL(shared_plan_kernel, dim3(1), dim3((unsigned)(need + 63) / 64 * 64), 0, s, pl);
+        else
+            hipLaunchKernelGGL(shared_plan_long_kernel, dim3(1), dim3(kPlanThreads), 0, s, pl);
+        VMC_LAUNCH_CHECK();
+    }
 
     TileParams p = {};
+    p.plan = pl;
+    p.fused = fused;
     p.out = a.out;
     p.q = a.q;
     p.q_ts = a.q_ts;
@@ -541,7 +375,6 @@ int shared_tiles(const SharedArgs& a, void* ws, hipStream_t s) {
     p.desc = pl.desc;
     p.range = pl.range;
     p.row = pl.row;
-    p.gs = pl.gs;
     p.ns = a.nsets;
     p.nsets = pl.nsets;
     p.paged = paged;

@@ -48,6 +48,12 @@ constexpr int kTileRows = 32 * kTileWaves;  // rows of an item (GGUF pages: half
 // lane at head_dim 64, 256 at 128, 512 at 256
 __host__ __device__ constexpr int tile_per_cu(int D) { return D == 64 ? 3 : D == 128 ? 2 : 1; }
 
+// Sets of a call whose plan every workgroup of the shared-keys kernel makes for itself, in
+// LDS (about the last size that leaves head_dim 64 its three workgroups a CU): the plan
+// kernel takes 5 to 8 us, this 2 to 3.  Not for whole items, of which a CU
+// takes one after the other, and each would plan again.
+constexpr int kPlanFused = 96;
+
 struct PlanParams {
     const int32_t* starts;
     const int32_t* set_lens;
@@ -77,8 +83,9 @@ struct TileParams {
     const SetDesc* desc;
     const RangeRec* range;
     const RowRec* row;
-    const int32_t* gs;
     int ns, nsets, paged, whole;
+    int fused;       // the kernel makes the plan itself
+    PlanParams plan;
     int total_rows;
     int grid, umin;  // ranges, and the fewest units of one
     float* part;     // partial rows of D + 4 floats: o, m, l, two unused

@@ -42,7 +42,7 @@
 #include "generic_row.hpp"
 #include "kv_quant.hpp"
 #include "prefill_dev.hpp"
-#include "shared_plan.hpp"
+#include "shared_plan_dev.hpp"
 
 namespace vmc {
 namespace {
@@ -150,7 +150,8 @@ __global__ void __launch_bounds__(256, tile_per_cu(D)) shared_tile_kernel(TilePa
     struct Lds {
         uint8_t tile[NS][2][TILE];                       // [slot][K, V]
         float qs[W][D];                                  // rows that rerun key by key
-        alignas(16) float vexp[2][W];                    // kConv [tile][16-key chunk]: 8 - log2 of V's scale
+        alignas(16) SetDesc desc[kPlanFused];            // (fused)
+        float vexp[2][W];                                // kConv [tile][16-key chunk]: 8 - log2 of V's scale
     };
     __shared__ __attribute__((aligned(1024))) Lds lds;
 
@@ -171,7 +172,12 @@ __global__ void __launch_bounds__(256, tile_per_cu(D)) shared_tile_kernel(TilePa
     struct Cursor {
         int set, g, rb, t, tiles, nb, klo, khi, src;
     };
+    auto uniform = [](const SetDesc& d) __attribute__((always_inline)) {
+        auto f = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+        return SetDesc{f(d.row0), f(d.ntok), f(d.klo), f(d.khi), f(d.src), f(d.nb), f(d.tiles), f(d.own)};
+    };
     auto desc_of = [&](int set) __attribute__((always_inline)) {
+        if (arg()->fused) return uniform(lds.desc[set]);
         const auto* s = as_const(reinterpret_cast<const int*>(arg()->desc + set));
         return SetDesc{s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7]};
     };
@@ -197,7 +203,10 @@ __global__ void __launch_bounds__(256, tile_per_cu(D)) shared_tile_kernel(TilePa
     Cursor cc;  // of the tile in use
     int range = blockIdx.x, units;
     SetDesc first;
-    if (arg()->whole) {  // one item; consecutive items to one XCD, whose L2 holds their keys
+    using Plan = PlanLds<kPlanFused, W>;
+    static_assert(sizeof(Plan) <= sizeof(lds.tile), "the plan's sums lie where tiles will");
+    Plan& plan = *reinterpret_cast<Plan*>(&lds.tile[0][0][0]);
+    if (p.whole) {  // one item; consecutive items to one XCD, whose L2 holds their keys
         const int64_t total = as_const(p.cum)[p.nsets], per = (total + 7) >> 3;
         const int64_t item = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
         if ((blockIdx.x >> 3) >= per || item >= total) return;
@@ -209,6 +218,27 @@ __global__ void __launch_bounds__(256, tile_per_cu(D)) shared_tile_kernel(TilePa
         cc.g = in_set / cc.nb;
         cc.rb = in_set % cc.nb;
         units = cc.tiles;
+    } else if (p.fused) {
+        const PlanSums sums = plan_sets(p.plan, plan, lds.desc, tid);
+        if (blockIdx.x == 0) plan_out(p.plan, sums, lds.desc, plan.cum, tid);
+        RangeRec r = {}, e;
+        const int n = plan_ranges(sums.total, p.grid, p.umin);
+        if (range < n) {
+            const int u0 = (int)div_floor<long long>((long long)range * sums.total, n);
+            const int u1 = (int)div_floor<long long>((long long)(range + 1) * sums.total, n);
+            r.ntiles = (u1 < sums.total ? range_begin(plan, lds.desc, p.nsets, u1, e) : sums.total_t);
+            r.ntiles -= range_begin(plan, lds.desc, p.nsets, u0, r);
+        }
+        if (tid == 0 && !p.paged) const_cast<RangeRec*>(p.range)[range] = r;  // (the merge's)
+        cc.set = __builtin_amdgcn_readfirstlane(r.set);
+        cc.g = __builtin_amdgcn_readfirstlane(r.g);
+        cc.rb = __builtin_amdgcn_readfirstlane(r.rb);
+        cc.t = __builtin_amdgcn_readfirstlane(r.t);
+        units = __builtin_amdgcn_readfirstlane(r.ntiles);
+        first = uniform(r.d);
+        take(cc, first);
+        if (units == 0) return;
+        __syncthreads();  // the plan's sums are read
     } else {
         const auto* r = as_const(reinterpret_cast<const int*>(p.range + range));
         cc.set = r[0];
