@@ -317,20 +317,16 @@ __global__ void __launch_bounds__(256, tile_per_cu(D)) shared_tile_kernel(TilePa
     };
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane(
         (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)&lds.tile[0][0][0]);
-    // offsets of this lane's rows in full tiles.  Row x of this wave's part, transfer i
-    auto part_row = [&](int i) __attribute__((always_inline)) { return kBN / W * w + i * (1024 / ROW) + lane / (D / 8); };
-    auto part_col = [&](int r) __attribute__((always_inline)) {
-        return 16u * (uint32_t)((lane % (D / 8)) ^ tile_swz<D>(r));
-    };
-    uint32_t off_k[kGguf ? 1 : NTR], off_v[SRC == TS_LOCAL ? NTR : 1];
-    if constexpr (!kGguf) {
-#pragma unroll
-        for (int i = 0; i < NTR; ++i) {
-            const int r = part_row(i);  // (paged: r & 15, the same for K and V)
-            off_k[i] = (uint32_t)(SRC == TS_LOCAL ? r : r & 15) * (uint32_t)p.k_row + part_col(r);
-            if constexpr (SRC == TS_LOCAL) off_v[i] = (uint32_t)r * (uint32_t)p.v_row + part_col(r);
-        }
-    }
+    // Row of the tile that transfer i of this wave brings to this lane, and its bytes' place
+    // in the row: the swizzle of rows TR i and the lane's own have no bit in common
+    constexpr int TR = 1024 / ROW;
+    int lane_row = lane / (D / 8);
+    uint32_t lane_col = 16u * (uint32_t)((lane % (D / 8)) ^ tile_swz<D>(lane_row));
+    auto part_row = [&](int i) __attribute__((always_inline)) { return kBN / W * w + TR * i + lane_row; };
+    auto part_col = [&](int i) __attribute__((always_inline)) { return lane_col ^ (16u * (uint32_t)tile_swz<D>(TR * i)); };
+    // (paged: of the row in its 16-key chunk, the same for K and V)
+    const uint32_t off_k = (uint32_t)part_row(0) % (SRC == TS_LOCAL ? kBN : 16) * (uint32_t)p.k_row;
+    const uint32_t off_v = SRC == TS_LOCAL ? (uint32_t)part_row(0) * (uint32_t)p.v_row : off_k;
     // this wave's part of K or V of a tile into LDS at dst
     auto transfer = [&](bool is_v, const Rec& x, uint32_t dst) __attribute__((always_inline)) {
         const uint64_t b64 = (uint64_t)(is_v ? p.vp + (SRC == TS_LOCAL ? x.v : x.k[0]) : p.kp + x.k[0]);
@@ -338,18 +334,22 @@ __global__ void __launch_bounds__(256, tile_per_cu(D)) shared_tile_kernel(TilePa
                                                (uint32_t)__builtin_amdgcn_readfirstlane((int)b64));
         const bool own_v = SRC == TS_LOCAL && is_v;
         dst += 1024u * NTR * (uint32_t)w;
+        const uint32_t step = (uint32_t)(own_v ? p.v_row : p.k_row);
+        // opaque, or the compiler computes every transfer's offset ahead, and where those fill
+        // the registers (head_dim 256) reads them from memory between transfers, behind a
+        // wait for all of them
+        if constexpr (D == 256) asm volatile("" : "+v"(lane_row), "+v"(lane_col));
         if (x.first == 0 && x.last >= kBN - 1) {
 #pragma unroll
             for (int i = 0; i < NTR; ++i)
-                dma16w(base, own_v ? off_v[SRC == TS_LOCAL ? i : 0] : off_k[kGguf ? 0 : i], dst + 1024u * i);
+                dma16w(base, (own_v ? off_v : off_k) + TR * i * step + part_col(i), dst + 1024u * i);
             return;
         }
-        const uint32_t step = (uint32_t)(own_v ? p.v_row : p.k_row);
 #pragma unroll
         for (int i = 0; i < NTR; ++i) {
             const int r = part_row(i);
             const int y = SRC == TS_LOCAL ? max(min(r, x.last), x.first) : chunk_row(r, x);
-            dma16w(base, (uint32_t)y * step + part_col(r), dst + 1024u * i);
+            dma16w(base, (uint32_t)y * step + part_col(i), dst + 1024u * i);
         }
     };
     uint32_t blk_raw[kGguf ? NBL : 1][kGguf ? NWD : 1];
