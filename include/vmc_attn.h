@@ -150,8 +150,13 @@ int vmc_paged_attention_decode(void* out, const void* query, const void* key_cac
  *                 length is, and the others through its own
  *   workspace     >= vmc_shared_prefix_workspace_size(...) bytes, 16-byte
  *                 aligned; calls that overlap on one workspace race
- * Any block_size.  The group arrays are read on the device: a captured call
- * follows their contents.  The size depends on the current device's CU count.
+ * batch * num_heads is below 2^24.  The group arrays are read on the device: a
+ * captured call follows their contents.  The size depends on the current
+ * device's CU count.  Any block_size: multiples of 16 with 16-byte aligned
+ * out, query and f16 / bf16 pages of q_dtype, or 4-byte aligned GGUF pages,
+ * run the MFMA kernel and its merge (two launches; with more than 96 rows and
+ * groups in all one before them, which plans), other shapes a
+ * one-wave-per-row kernel.
  */
 size_t vmc_shared_prefix_workspace_size(int batch_size, int num_heads, int num_kv_heads,
                                         int head_dim, int num_groups);
@@ -183,9 +188,13 @@ int vmc_paged_attention_shared_prefix(void* out, const void* query, const void* 
  *                 (share states), and lie packed or padded
  *   workspace     >= vmc_cross_attention_workspace_size(...) bytes, 16-byte
  *                 aligned; calls that overlap on one workspace race
- * Strides are even and at least head_dim, key and value 4-byte aligned.  The
- * starts and lengths are read on the device: a captured call follows their
- * contents.  The size depends on the current device's CU count.
+ * num_tokens is below 2^24, num_tokens * num_heads below 2^31.  Strides are
+ * even and at least head_dim, key and value 4-byte aligned.  The starts and
+ * lengths are read on the device: a captured call follows their contents.  The
+ * size depends on the current device's CU count.  With all tensors 16-byte
+ * aligned and strides in multiples of 8 the MFMA kernel runs (with its merge,
+ * or, for many rows, a plan before it; both from 97 sequences on), else a
+ * one-wave-per-row kernel.
  */
 size_t vmc_cross_attention_workspace_size(int num_tokens, int num_seqs, int num_heads,
                                           int num_kv_heads, int head_dim);

@@ -31,15 +31,17 @@ def _rope(lib, **kw):
 PREFIX = [dict(batch=-1), dict(groups=-1), dict(hq=0), dict(hkv=0), dict(hkv=3), dict(d=96), dict(bs=0), dict(bs=-16),
           dict(blocks=-1), dict(blocks=1 << 28), dict(qt=2), dict(fmt=4), dict(fmt=-1), dict(layout=2), dict(out=None),
           dict(q=None), dict(k=None), dict(v=None), dict(bt=None), dict(lens=None), dict(starts=None),
-          dict(shared=None), dict(k=C.c_void_p(4098)), dict(v=C.c_void_p(4097), fmt=2), dict(out=C.c_void_p(4097))]
+          dict(shared=None), dict(k=C.c_void_p(4098)), dict(v=C.c_void_p(4097), fmt=2), dict(out=C.c_void_p(4097)),
+          dict(batch=1 << 21)]
 CROSS = [dict(t=-1), dict(n=-1), dict(s=-1), dict(hq=7), dict(d=80), dict(q_ts=127), dict(k_hs=64), dict(v_ts=257),
          dict(k_ts=-256), dict(dt=2), dict(out=None), dict(q=None), dict(k=None), dict(v=None), dict(qs=None),
-         dict(ks=None), dict(kl=None), dict(k=C.c_void_p(4098))]
+         dict(ks=None), dict(kl=None), dict(k=C.c_void_p(4098)), dict(t=1 << 24), dict(t=1 << 23, hq=256)]
 ROPE = [dict(d=96), dict(rot=0), dict(rot=24), dict(rot=144), dict(t=-1), dict(hq=0), dict(hkv=0), dict(max_pos=0),
         dict(dt=2), dict(q_ts=1000), dict(q_ts=1028), dict(k_ts=248), dict(v_ts=260), dict(q_out=None), dict(q=None),
         dict(k=None), dict(v=None), dict(cs=None), dict(pos=None), dict(kc=None), dict(vc=None), dict(slots=None),
         dict(bs=0), dict(fmt=4), dict(layout=2), dict(stride=16 * 2 * 256 - 16), dict(stride=16 * 2 * 256 + 8),
-        dict(q=C.c_void_p(4104)), dict(kc=C.c_void_p(4104)), dict(kc=C.c_void_p(4097), fmt=2)]
+        dict(q=C.c_void_p(4104)), dict(kc=C.c_void_p(4104)), dict(kc=C.c_void_p(4097), fmt=2),
+        dict(t=1 << 27)]
 
 
 @pytest.mark.parametrize("call,cases", [(_prefix, PREFIX), (_cross, CROSS), (_rope, ROPE)])

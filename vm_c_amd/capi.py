@@ -387,7 +387,8 @@ def _int32(what, n, **tensors):
 def _on_current_device(t, what):
     """A kernel runs on the current device: memory of another one is not its own."""
     import torch
-    if t.device.type != "cuda" or t.device.index != torch.cuda.current_device():
+    d = t.get_device()  # -1: host memory
+    if d < 0 or d != torch._C._cuda_getDevice():
         raise VmcError(f"{what}: tensors are on {t.device}, not on the current device")
 
 

@@ -8,10 +8,11 @@
 // What bounds it: HBM for a prefill step, the launch and its dependent reads
 // (position -> table row) for a decode step.  A head's row is D / 8 lanes of 16
 // bytes; the lanes of a row exchange the pairs' other halves, so each value is
-// read and written once.  The same lanes take R heads of one token, whose loads
-// are all issued before the first is used and which share the table row: the
-// table is the widest read of a head (rotary_dim fp32 against head_dim 16-bit
-// values).
+// read and written once; the table rows come from the L2.  Measured: 65 us for 16384
+// tokens of 16 + 2 heads of 256 with their V (0.34 GB in and out, 5.2 TB/s, what a
+// copy reaches), 7.4 us for 5003 tokens of 14 + 2 heads of 64, 3.4 us for 32
+// tokens.  Several heads a lane, sharing a table row, would save reads
+// that the L2 has anyway.
 #include "row_codec.hpp"
 
 namespace vmc {
@@ -37,35 +38,32 @@ struct RopeParams {
 
 constexpr int kNoPages = -1;
 
-// Rows of a token: Hkv K rows (with their V rows), then Hq Q rows, R at a time
-// (R divides both counts).  FMT: page format, or kNoPages.
-template <int D, bool BF, int FMT, bool NEOX, int R>
+// Rows of a token: Hkv K rows (with their V rows), then Hq Q rows.  FMT: page format,
+// or kNoPages.
+template <int D, bool BF, int FMT, bool NEOX>
 __global__ void __launch_bounds__(256) rope_append_kernel(RopeParams p) {
     constexpr int LPR = D / 8;      // lanes of a row
-    constexpr int GPW = 256 / LPR;  // row groups of a workgroup
+    constexpr int RPW = 256 / LPR;  // rows of a workgroup
     const int j = threadIdx.x % LPR;
-    const int per_tok = (p.Hkv + p.Hq) / R;
-    const int64_t item = (int64_t)blockIdx.x * GPW + threadIdx.x / LPR;
+    const uint32_t per_tok = (uint32_t)(p.Hkv + p.Hq);
+    const uint32_t item = blockIdx.x * RPW + threadIdx.x / LPR;
     const int64_t t_raw = item / per_tok;
     // lanes past the end follow the last token without writing (they take part
     // in the exchanges of their wave)
     const int64_t t = min(t_raw, (int64_t)p.T - 1);
-    const int r0 = (int)(item % per_tok) * R;
-    const bool is_k = r0 < p.Hkv;
-    const int h0 = is_k ? r0 : r0 - p.Hkv;
+    const int row = (int)(item % per_tok);
+    const bool is_k = row < p.Hkv;
+    const int h = is_k ? row : row - p.Hkv;
 
     const int64_t pos = p.pos[t];
     const bool live = t_raw < p.T && pos >= 0 && pos < p.max_pos;
-    const uint16_t* src = (is_k ? p.k + t * p.k_ts : p.q + t * p.q_ts) + (int64_t)h0 * D + 8 * j;
-    u32x4 xr[R], vr[R];
-#pragma unroll
-    for (int r = 0; r < R; ++r) xr[r] = *reinterpret_cast<const u32x4*>(src + r * D);
+    const uint16_t* src = (is_k ? p.k + t * p.k_ts : p.q + t * p.q_ts) + (int64_t)h * D + 8 * j;
+    const u32x4 xr = *reinterpret_cast<const u32x4*>(src);
+    u32x4 vr = {0u, 0u, 0u, 0u};
     int64_t slot = -1;
     if constexpr (FMT != kNoPages) {
         if (is_k) {
-            const uint16_t* vs = p.v + t * p.v_ts + (int64_t)h0 * D + 8 * j;
-#pragma unroll
-            for (int r = 0; r < R; ++r) vr[r] = *reinterpret_cast<const u32x4*>(vs + r * D);
+            vr = *reinterpret_cast<const u32x4*>(p.v + t * p.v_ts + (int64_t)h * D + 8 * j);
             if (live) slot = p.slots[t];
         }
     }
@@ -78,12 +76,12 @@ __global__ void __launch_bounds__(256) rope_append_kernel(RopeParams p) {
     constexpr int NC = NEOX ? 8 : 4;
     float c[NC], s[NC];
     {
-        const float* row = p.cs + (live ? pos : 0) * p.rot;
+        const float* cs = p.cs + (live ? pos : 0) * p.rot;
         const int at = turns ? (NEOX ? 8 * (lower ? j - hc : j) : 4 * j) : 0;
 #pragma unroll
         for (int e = 0; e < NC; e += 4) {
-            const f32x4 cv = *reinterpret_cast<const f32x4*>(row + at + e);
-            const f32x4 sv = *reinterpret_cast<const f32x4*>(row + half + at + e);
+            const f32x4 cv = *reinterpret_cast<const f32x4*>(cs + at + e);
+            const f32x4 sv = *reinterpret_cast<const f32x4*>(cs + half + at + e);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 c[e + i] = cv[i];
@@ -92,70 +90,66 @@ __global__ void __launch_bounds__(256) rope_append_kernel(RopeParams p) {
         }
     }
     const int mate_lane = (int)(threadIdx.x & 63) - j + mate;
+    float x[8], y[8];
+    unpack8<BF>(xr, x);
+    if constexpr (NEOX) {
+        u32x4 ow;
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        float x[8], y[8];
-        unpack8<BF>(xr[r], x);
-        if constexpr (NEOX) {
-            u32x4 ow;
+        for (int e = 0; e < 4; ++e) ow[e] = (uint32_t)__shfl((int)xr[e], mate_lane, kWave);
+        float o[8];
+        unpack8<BF>(ow, o);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) ow[e] = (uint32_t)__shfl((int)xr[r][e], mate_lane, kWave);
-            float o[8];
-            unpack8<BF>(ow, o);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float t0 = x[e] * c[e], t1 = o[e] * s[e];
-                y[e] = lower ? t0 + t1 : t0 - t1;
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float a = x[2 * i], b = x[2 * i + 1];
-                y[2 * i] = a * c[i] - b * s[i];
-                y[2 * i + 1] = b * c[i] + a * s[i];
-            }
+        for (int e = 0; e < 8; ++e) {
+            const float t0 = x[e] * c[e], t1 = o[e] * s[e];
+            y[e] = lower ? t0 + t1 : t0 - t1;
         }
-        const u32x4 turned = pack8<BF>(y);
-        const u32x4 yw = turns ? turned : xr[r];  // values that do not turn keep their bits
-        const int64_t at = (t * (is_k ? p.Hkv : p.Hq) + h0 + r) * D + 8 * j;
-        uint16_t* dst = is_k ? p.k_out : p.q_out;
-        if (live && dst) *reinterpret_cast<u32x4*>(dst + at) = yw;
-        if constexpr (FMT != kNoPages) {
-            if (!is_k) continue;
-            const bool wr = slot >= 0;
-            const int64_t eo = kv_entry_offset(wr ? slot : 0, h0 + r, p.bs, p.Hkv, p.E, p.stride, p.hnd != 0);
-            if constexpr (FMT == VMC_KV_F16 || FMT == VMC_KV_BF16) {
-                constexpr bool DB = FMT == VMC_KV_BF16;
-                u32x4 kw = yw, vw = vr[r];
-                if constexpr (DB != BF) {
-                    float f[8];
-                    unpack8<BF>(yw, f);
-                    kw = pack8<DB>(f);
-                    unpack8<BF>(vr[r], f);
-                    vw = pack8<DB>(f);
-                }
-                if (wr) {
-                    *reinterpret_cast<u32x4*>(p.kc + eo + 16 * j) = kw;
-                    *reinterpret_cast<u32x4*>(p.vc + eo + 16 * j) = vw;
-                }
-            } else {
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float a = x[2 * i], b = x[2 * i + 1];
+            y[2 * i] = a * c[i] - b * s[i];
+            y[2 * i + 1] = b * c[i] + a * s[i];
+        }
+    }
+    const u32x4 turned = pack8<BF>(y);
+    const u32x4 yw = turns ? turned : xr;  // values that do not turn keep their bits
+    const int64_t at = (t * (is_k ? p.Hkv : p.Hq) + h) * D + 8 * j;
+    uint16_t* dst = is_k ? p.k_out : p.q_out;
+    if (live && dst) *reinterpret_cast<u32x4*>(dst + at) = yw;
+    if constexpr (FMT != kNoPages) {
+        if (!is_k) return;
+        const bool wr = slot >= 0;
+        const int64_t eo = kv_entry_offset(wr ? slot : 0, h, p.bs, p.Hkv, p.E, p.stride, p.hnd != 0);
+        if constexpr (FMT == VMC_KV_F16 || FMT == VMC_KV_BF16) {
+            constexpr bool DB = FMT == VMC_KV_BF16;
+            u32x4 kw = yw, vw = vr;
+            if constexpr (DB != BF) {
                 float f[8];
                 unpack8<BF>(yw, f);
-                gguf_block4<FMT>(f, j, p.kc + eo, wr);
-                unpack8<BF>(vr[r], f);
-                gguf_block4<FMT>(f, j, p.vc + eo, wr);
+                kw = pack8<DB>(f);
+                unpack8<BF>(vr, f);
+                vw = pack8<DB>(f);
             }
+            if (wr) {
+                *reinterpret_cast<u32x4*>(p.kc + eo + 16 * j) = kw;
+                *reinterpret_cast<u32x4*>(p.vc + eo + 16 * j) = vw;
+            }
+        } else {
+            float f[8];
+            unpack8<BF>(yw, f);
+            gguf_block4<FMT>(f, j, p.kc + eo, wr);
+            unpack8<BF>(vr, f);
+            gguf_block4<FMT>(f, j, p.vc + eo, wr);
         }
     }
 }
 
 template <int D, bool BF, int FMT, bool NEOX>
 int launch_rope(const RopeParams& p, hipStream_t s) {
-    const int R = 1;
-    const int64_t items = (int64_t)p.T * ((p.Hkv + p.Hq) / R);
+    const int64_t items = (int64_t)p.T * ((int64_t)p.Hkv + p.Hq);
+    if (items >= ((int64_t)1 << 32) / (D / 8) - 256) return VMC_EINVAL;  // a launch has 2^32 work-items at most
     const int64_t grid = (items + 256 / (D / 8) - 1) / (256 / (D / 8));
-    if (grid > 0x7fffffff) return VMC_EINVAL;
-    hipLaunchKernelGGL((rope_append_kernel<D, BF, FMT, NEOX, 1>), dim3((unsigned)grid), dim3(256), 0, s, p);
+    hipLaunchKernelGGL((rope_append_kernel<D, BF, FMT, NEOX>), dim3((unsigned)grid), dim3(256), 0, s, p);
     VMC_LAUNCH_CHECK();
     return VMC_OK;
 }

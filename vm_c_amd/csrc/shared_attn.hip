@@ -140,6 +140,7 @@ extern "C" int vmc_paged_attention_shared_prefix(void* out, const void* query, c
     const int64_t entry = vmc_kv_entry_bytes(kv_format, head_dim);
     if (entry < 0) return VMC_EINVAL;
     if (batch_size == 0) return VMC_OK;
+    if ((int64_t)batch_size * num_heads >= 1 << 24) return VMC_EINVAL;  // 2^32 work-items of 256 a row and head
     if (!out || !query || !key_cache || !value_cache || !block_tables || !seq_lens) return VMC_EINVAL;
     if (num_groups > 0 && (!group_starts || !shared_lens)) return VMC_EINVAL;
     // entries are read as 32-bit words (f16 / bf16) or 16-bit ones (GGUF)
@@ -198,6 +199,7 @@ extern "C" int vmc_cross_attention(void* out, const void* query, const void* key
                        value_head_stride})
         if (st < head_dim || st % 2 != 0 || st > (int64_t)1 << 40) return VMC_EINVAL;
     if (num_tokens == 0 || num_seqs == 0) return VMC_OK;
+    if (num_tokens >= 1 << 24 || (int64_t)num_tokens * num_heads > 0x7fffffff) return VMC_EINVAL;
     if (!out || !query || !query_starts || !key_starts || !key_lens) return VMC_EINVAL;
     if (num_keys > 0 && (!key || !value)) return VMC_EINVAL;
     if ((((uintptr_t)out | (uintptr_t)query) & 1) != 0 || (((uintptr_t)key | (uintptr_t)value) & 3) != 0)

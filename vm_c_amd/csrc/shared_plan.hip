@@ -288,7 +288,7 @@ Shape shape_of(bool paged, int rows, int nsets, int Hq, int Hkv, int D) {
     sh.grid = num_cus() * tile_per_cu(D);
     // Whole items where sets of many rows give several times the workgroups
     const int64_t items = (int64_t)Hkv * (rows * G / kTileRows + std::min<int64_t>(rows, sets));
-    if (!paged && rows * G >= kTileRows * sets && items >= 4 * (int64_t)sh.grid && items < (1 << 30)) {
+    if (!paged && rows * G >= kTileRows * sets && items >= 4 * (int64_t)sh.grid && items < (1 << 24)) {
         sh.whole = 1;
         sh.grid = (int)((items + 7) & ~7);
     }
