@@ -11,6 +11,7 @@
 
 #include "vm_c/attention_backend.hpp"
 #include "vm_c/attention_metadata.hpp"
+#include "vm_c/kernels_fused_attn.hpp"
 #include "vm_c/kv_cache_manager.hpp"
 #include "vm_c/turboquant_kv_bridge.hpp"
 
@@ -429,6 +430,106 @@ static void test_tq_bridge() {
     CHECK(ws.decode_workspace == nullptr && ws.decode_bytes == 0);
 }
 
+// Rows of a decode batch that begin with the same whole blocks, in groups
+static void test_shared_prefix_groups() {
+    HostBatchMetadata h;
+    auto batch = [&](const std::vector<std::vector<int32_t>>& rows, const std::vector<int32_t>& lens) {
+        h = HostBatchMetadata{};
+        h.num_reqs = h.num_decodes = (int)rows.size();
+        for (auto& r : rows) h.max_num_blocks_per_req = std::max(h.max_num_blocks_per_req, (int)r.size());
+        for (auto& r : rows)
+            for (int i = 0; i < h.max_num_blocks_per_req; ++i)
+                h.block_tables.push_back(i < (int)r.size() ? r[i] : -1);
+        h.seq_lens = lens;
+    };
+    using V = std::vector<int32_t>;
+    // two rows of three common blocks, one alone, two whose common block is the second one only
+    batch({{1, 2, 3, 4}, {1, 2, 3, 5}, {6, 7}, {8, 9}, {10, 9}}, {60, 64, 20, 30, 30});
+    CHECK(group_shared_prefixes(h, 16) == 48);
+    CHECK((h.prefix_group_starts == V{0, 2, 3, 4, 5}) && (h.shared_prefix_lens == V{48, 0, 0, 0}));
+    CHECK(group_shared_prefixes(h, 16, 49) == 0 && h.prefix_group_starts.empty() && h.shared_prefix_lens.empty());
+    // only whole blocks of both rows count: 47 tokens have two
+    batch({{1, 2, 3}, {1, 2, 3}}, {47, 48});
+    CHECK(group_shared_prefixes(h, 16) == 32);
+    CHECK((h.shared_prefix_lens == V{32}));
+    // a third row with a shorter prefix joins where that saves no less (2 * 1 against 1 * 2 blocks),
+    // and stays out where it would (2 * 1 against 1 * 3)
+    batch({{1, 2, 3, 4}, {1, 2, 5, 6}, {1, 7, 8, 9}}, {64, 64, 64});
+    CHECK(group_shared_prefixes(h, 16) == 32 && (h.prefix_group_starts == V{0, 3}) && (h.shared_prefix_lens == V{16}));
+    batch({{1, 2, 3, 4}, {1, 2, 3, 6}, {1, 7, 8, 9}}, {64, 64, 64});
+    CHECK(group_shared_prefixes(h, 16) == 48 && (h.prefix_group_starts == V{0, 2, 3}) &&
+          (h.shared_prefix_lens == V{48, 0}));
+    // holes end a prefix; nothing shared, one row, a prefill row: no groups
+    batch({{1, -1, 3}, {1, -1, 3}}, {48, 48});
+    CHECK(group_shared_prefixes(h, 16) == 16);
+    batch({{1}, {2}}, {16, 16});
+    CHECK(group_shared_prefixes(h, 16) == 0 && h.prefix_group_starts.empty());
+    batch({{1, 2}}, {32});
+    CHECK(group_shared_prefixes(h, 16) == 0);
+    batch({{1, 2}, {1, 2}}, {32, 32});
+    h.num_prefills = 1;
+    CHECK(group_shared_prefixes(h, 16) == 0);
+    bool threw = false;
+    try {
+        group_shared_prefixes(h, 0);
+    } catch (const std::runtime_error&) {
+        threw = true;
+    }
+    CHECK(threw);
+    // rows that a manager hands the same cached blocks
+    KVCacheManager m(cache_cfg(), ModelConfig{}, 1, 8, 128, 0, false, hostmem());
+    m.allocate_gpu_blocks_for_group(0, 32);
+    std::vector<int64_t> ids;
+    for (auto& s : m.allocate_slots("a", 40)) ids.push_back(s.block_id);
+    std::vector<ScheduledRequest> reqs(2);
+    reqs[0].request_id = "a";
+    reqs[0].num_computed_tokens = 40;
+    reqs[1].request_id = "b";
+    reqs[1].num_computed_tokens = 33;
+    reqs[1].num_cached_tokens = 32;
+    reqs[1].computed_block_ids = {ids[0], ids[1]};
+    h = build_batch_metadata(m, reqs);
+    CHECK(h.ok);
+    const bool shared = h.block_tables[0] == h.block_tables[h.max_num_blocks_per_req];
+    CHECK(group_shared_prefixes(h, 16) == (shared ? 32 : 0));
+}
+
+// What the shared-prefix decode, the cross attention and the rotation with append refuse
+static void test_shared_attention_errors() {
+    auto refused = [](const std::function<void()>& f) {
+        try {
+            f();
+        } catch (const std::runtime_error& e) {
+            return std::string(e.what()).find("invalid argument") != std::string::npos;
+        }
+        return false;
+    };
+    AttentionParams p;
+    p.batch_size = 2;
+    p.num_heads = 8;
+    p.num_kv_heads = 3;  // does not divide 8
+    p.head_dim = 128;
+    p.block_size = 16;
+    p.max_num_blocks_per_req = 4;
+    CHECK(refused([&] {
+        paged_attention_shared_prefix(nullptr, nullptr, 0, nullptr, nullptr, nullptr, p, nullptr, nullptr, nullptr, nullptr,
+                                      0, "fp16");
+    }));
+    CHECK(paged_attention_shared_prefix_workspace_size(p, 1) == 0);
+    CrossAttentionParams c;
+    c.num_tokens = c.num_keys = c.num_seqs = 1;
+    c.num_heads = c.num_kv_heads = 4;
+    c.head_dim = 96;
+    CHECK(refused([&] { cross_attention(nullptr, nullptr, 0, nullptr, nullptr, nullptr, c, nullptr, nullptr, nullptr); }));
+    c.head_dim = 64;
+    c.key_token_stride = 63;
+    CHECK(refused([&] { cross_attention(nullptr, nullptr, 0, nullptr, nullptr, nullptr, c, nullptr, nullptr, nullptr); }));
+    CHECK(refused([&] {
+        rope_and_cache(nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, 1, 4, 4, 64,
+                       24, 10, 0, 0, 0, true, 16, 0, "fp16");
+    }));
+}
+
 int main() {
     const std::vector<std::pair<const char*, std::function<void()>>> tests = {
         {"free_queue", test_free_queue},
@@ -441,6 +542,8 @@ int main() {
         {"metadata", test_metadata},
         {"errors", test_errors},
         {"tq_bridge", test_tq_bridge},
+        {"shared_prefix_groups", test_shared_prefix_groups},
+        {"shared_attention_errors", test_shared_attention_errors},
     };
     for (auto& t : tests) {
         const int before = g_fail;

@@ -602,6 +602,178 @@ static void test_tq_bridge_node(const char* method) {
     for (const char* id : {"r0", "r1", "r2", "r3"}) mgr.free_slots(id);
 }
 
+// A decode step of requests that share a prefix through the backend: the step's Q, K, V
+// rotated and appended from one projection (rope_and_cache), rows grouped by
+// their blocks (group_shared_prefixes), forward_decode over the groups, then the
+// rows' cross attention over an encoder's states.
+static void test_shared_prefix_step(const std::string& dtype, const std::string& layout) {
+    std::printf("case: shared prefix step %s %s\n", dtype.c_str(), layout.c_str());
+    std::fflush(stdout);
+    CacheConfig cc;
+    cc.kv_cache_dtype = dtype;
+    cc.kv_cache_layout = layout;
+    KVCacheManager mgr(cc, ModelConfig{}, 1, Hkv, D);
+    mgr.allocate_gpu_blocks_for_group(0, 128);
+    PagedAttentionBackend be(layout, dtype, ScalarType::FLOAT16);
+    be.ensure_workspace(1024, 8, Hq, Hkv, D, 0);
+    const std::vector<int> lens = {301, 160, 222, 18, 1};  // tokens in the cache before the step
+    const int R = (int)lens.size(), shared = 9;            // rows 0 .. 2 share 9 blocks
+    std::vector<ScheduledRequest> rq(R);
+    for (int i = 0; i < R; ++i) {
+        rq[i].request_id = "s" + std::to_string(i);
+        rq[i].num_scheduled_tokens = lens[i];
+        rq[i].is_prefill = true;
+    }
+    HostBatchMetadata hp = build_batch_metadata(mgr, rq);
+    CHECK(hp.ok);
+    std::vector<uint16_t> K((size_t)hp.num_tokens * Hkv * D), V(K.size());
+    orc_randn_f16(K.data(), (int64_t)K.size(), 19, 1);
+    orc_randn_f16(V.data(), (int64_t)V.size(), 19, 2);
+    Dev<uint16_t> dK(K), dV(V);
+    DeviceBatchMetadata dm(8, 1024, 96);
+    AttentionMetadata mp = dm.upload(hp, BS, nullptr);
+    const size_t pool_n = (size_t)128 * mgr.group(0).bytes_per_block;
+    HIP_CHECK(hipMemset(mgr.key_cache_ptr(0), 0, pool_n));
+    HIP_CHECK(hipMemset(mgr.value_cache_ptr(0), 0, pool_n));
+    be.store_kv(dK.p, dV.p, mgr.key_cache_ptr(0), mgr.value_cache_ptr(0), mp.slot_mapping, hp.num_tokens, Hkv, D, BS, 0,
+                nullptr);
+    HIP_CHECK(hipDeviceSynchronize());
+    for (int i = 0; i < R; ++i) {
+        rq[i].num_computed_tokens = lens[i];
+        rq[i].num_scheduled_tokens = 1;
+        rq[i].is_prefill = false;
+    }
+    HostBatchMetadata h = build_batch_metadata(mgr, rq);
+    CHECK(h.ok);
+    const int mb = h.max_num_blocks_per_req;
+    for (int r : {1, 2}) std::copy_n(h.block_tables.begin(), shared, h.block_tables.begin() + (size_t)r * mb);
+    CHECK(group_shared_prefixes(h, BS) == 2 * shared * BS);
+    CHECK((h.prefix_group_starts == std::vector<int32_t>{0, 3, 4, 5}));
+    CHECK((h.shared_prefix_lens == std::vector<int32_t>{shared * BS, 0, 0}));
+    AttentionMetadata md = dm.upload(h, BS, nullptr);
+    CHECK(md.num_prefix_groups == 3);
+
+    // the projection's rows [Q | K | V], half of each head rotated
+    const int W = (Hq + 2 * Hkv) * D, rot = 64, maxpos = 512;
+    std::vector<uint16_t> qkv((size_t)R * W);
+    orc_randn_f16(qkv.data(), (int64_t)qkv.size(), 19, 3);
+    std::vector<float> cs((size_t)maxpos * rot);
+    for (int p = 0; p < maxpos; ++p)
+        for (int i = 0; i < rot / 2; ++i) {
+            const double a = p * std::pow(10000.0, -2.0 * i / rot);
+            cs[(size_t)p * rot + i] = (float)std::cos(a);
+            cs[(size_t)p * rot + rot / 2 + i] = (float)std::sin(a);
+        }
+    std::vector<int64_t> pos(lens.begin(), lens.end());
+    Dev<uint16_t> dqkv(qkv), dQ((size_t)R * Hq * D), dKo((size_t)R * Hkv * D), dO((size_t)R * Hq * D);
+    Dev<float> dcs(cs);
+    Dev<int64_t> dpos(pos);
+    rope_and_cache(dQ.p, dKo.p, dqkv.p, dqkv.p + Hq * D, dqkv.p + (Hq + Hkv) * D, dcs.p, dpos.p, mgr.key_cache_ptr(0),
+                   mgr.value_cache_ptr(0), md.slot_mapping, R, Hq, Hkv, D, rot, maxpos, W, W, W, true, BS, 0, dtype,
+                   nullptr, ScalarType::FLOAT16, layout);
+    HIP_CHECK(hipDeviceSynchronize());
+    std::vector<uint16_t> Q = dQ.get(), Ko = dKo.get();
+    bool turned = true;
+    for (int r = 0; r < R; ++r)
+        for (int hd = 0; hd < Hq + Hkv; ++hd)
+            for (int i = 0; i < D; ++i) {
+                const uint16_t* x = &qkv[(size_t)r * W + hd * D];
+                const int m = i < rot / 2 ? i + rot / 2 : i - rot / 2;
+                const double a = orc_f16_to_f32(x[i]);
+                const float* c = &cs[(size_t)pos[r] * rot];
+                const double want = i >= rot ? a
+                                    : i < rot / 2 ? a * c[i] - orc_f16_to_f32(x[m]) * c[rot / 2 + i]
+                                                  : a * c[m] + orc_f16_to_f32(x[m]) * c[rot / 2 + m];
+                const double got = orc_f16_to_f32(hd < Hq ? Q[((size_t)r * Hq + hd) * D + i]
+                                                          : Ko[((size_t)r * Hkv + hd - Hq) * D + i]);
+                // one rounding to fp16, fp32 products before it
+                turned = turned && std::fabs(got - want) <= std::ldexp(std::fabs(want), -11) + 1e-6;
+            }
+    CHECK(turned);
+    // the pages hold what an append of the rotated K and of V writes
+    std::vector<uint8_t> gk = pool_bytes(mgr.key_cache_ptr(0), pool_n), gv = pool_bytes(mgr.value_cache_ptr(0), pool_n);
+    const int fmt = dtype == "q8_0" ? ORC_KV_Q8_0 : dtype == "q4_0" ? ORC_KV_Q4_0 : ORC_KV_F16;
+    std::vector<uint16_t> Vs;
+    for (int r = 0; r < R; ++r)
+        Vs.insert(Vs.end(), qkv.begin() + (size_t)r * W + (Hq + Hkv) * D, qkv.begin() + (size_t)(r + 1) * W);
+    std::vector<uint8_t> rk = gk, rv = gv;
+    orc_kv_append(Ko.data(), Vs.data(), 0, rk.data(), rv.data(), h.slot_mapping.data(), R, Hkv, D, BS, fmt, layout == "hnd");
+    CHECK(gk == rk && gv == rv);
+
+    std::vector<float> qf(Q.size());
+    orc_f16_to_f32_n(Q.data(), qf.data(), (int64_t)Q.size());
+    std::vector<double> ex(Q.size());
+    const double scale = 1.0 / std::sqrt((double)D);
+    orc_paged_decode_exact(ex.data(), qf.data(), gk.data(), gv.data(), fmt, layout == "hnd", h.block_tables.data(),
+                           h.seq_lens.data(), R, Hq, Hkv, D, scale, BS, mb, 0);
+    double err = 0;
+    for (int groups : {3, 0}) {
+        md.num_prefix_groups = groups;
+        HIP_CHECK(hipMemset(dO.p, 0xff, sizeof(uint16_t) * dO.n));
+        be.forward_decode(dO.p, dQ.p, mgr.key_cache_ptr(0), mgr.value_cache_ptr(0), md, Hq, Hkv, D, (float)scale, BS,
+                          ScalarType::FLOAT16, nullptr);
+        HIP_CHECK(hipDeviceSynchronize());
+        CHECK(close(dO.get(), ex, &err));
+        std::printf("  decode, %d groups: max err %.3g\n", groups, err);
+    }
+    // a backend whose workspace was made for fewer rows reads each row's own
+    PagedAttentionBackend bare(layout, dtype, ScalarType::FLOAT16);
+    md.num_prefix_groups = 3;
+    bare.forward_decode(dO.p, dQ.p, mgr.key_cache_ptr(0), mgr.value_cache_ptr(0), md, Hq, Hkv, D, (float)scale, BS,
+                        ScalarType::FLOAT16, nullptr);
+    HIP_CHECK(hipDeviceSynchronize());
+    CHECK(close(dO.get(), ex, &err));
+
+    // rows 0, 1 over states 0 .. 69, rows 2 .. 4 over states 70 .. 102
+    const int N = 103;
+    std::vector<uint16_t> S((size_t)N * 2 * Hkv * D);
+    orc_randn_f16(S.data(), (int64_t)S.size(), 19, 4);
+    Dev<uint16_t> dS(S), dC((size_t)R * Hq * D);
+    Dev<int32_t> qs(std::vector<int32_t>{0, 2, 5}), ks(std::vector<int32_t>{0, 70}), kl(std::vector<int32_t>{70, 33});
+    CrossAttentionParams cp;
+    cp.num_tokens = R;
+    cp.num_keys = N;
+    cp.num_seqs = 2;
+    cp.num_heads = Hq;
+    cp.num_kv_heads = Hkv;
+    cp.head_dim = D;
+    cp.key_token_stride = cp.value_token_stride = 2 * Hkv * D;  // K and V of one projection
+    cp.scale = (float)scale;
+    const size_t need = cross_attention_workspace_size(cp);
+    Dev<uint8_t> ws(need);
+    bool small = false;
+    try {
+        cross_attention(dC.p, ws.p, need - 1, dO.p, dS.p, dS.p + Hkv * D, cp, qs.p, ks.p, kl.p);
+    } catch (const std::runtime_error&) {
+        small = true;
+    }
+    CHECK(small);
+    cross_attention(dC.p, ws.p, need, dO.p, dS.p, dS.p + Hkv * D, cp, qs.p, ks.p, kl.p);
+    HIP_CHECK(hipDeviceSynchronize());
+    const std::vector<uint16_t> X = dO.get();
+    std::vector<double> want((size_t)R * Hq * D, 0.0);
+    for (int r = 0; r < R; ++r)
+        for (int hd = 0; hd < Hq; ++hd) {
+            const int k0 = r < 2 ? 0 : 70, n = r < 2 ? 70 : 33, g = hd / (Hq / Hkv);
+            std::vector<double> s(n);
+            double m = -1e300, l = 0;
+            for (int k = 0; k < n; ++k) {
+                for (int i = 0; i < D; ++i)
+                    s[k] += (double)orc_f16_to_f32(X[((size_t)r * Hq + hd) * D + i]) *
+                            orc_f16_to_f32(S[((size_t)(k0 + k) * 2 * Hkv + g) * D + i]);
+                s[k] *= scale;
+                m = std::max(m, s[k]);
+            }
+            for (int k = 0; k < n; ++k) l += s[k] = std::exp(s[k] - m);
+            for (int k = 0; k < n; ++k)
+                for (int i = 0; i < D; ++i)
+                    want[((size_t)r * Hq + hd) * D + i] +=
+                        s[k] / l * orc_f16_to_f32(S[((size_t)(k0 + k) * 2 * Hkv + Hkv + g) * D + i]);
+        }
+    CHECK(close(dC.get(), want, &err));
+    std::printf("  cross attention max err %.3g\n", err);
+}
+
 int main() {
     int n = 0;
     if (hipGetDeviceCount(&n) != hipSuccess || n < 1) {
@@ -619,6 +791,8 @@ int main() {
         test_fused_norm_rope("q4_0");
         test_fused_norm_rope("auto");
         test_page_movement();
+        test_shared_prefix_step("q8_0", "nhd");
+        test_shared_prefix_step("fp16", "hnd");
         // (turboquant_k3v4_nc: skipped.  A run of this binary ended with
         // SIGSEGV inside that case, before its first step reported, after
         // changes to code the case does not call (fp8 page appends); the

@@ -32,6 +32,13 @@ struct AttentionMetadata {
     int num_decode_tokens = 0;
     bool is_prefill = false;
     float decode_threshold = 0.0f;
+    // Decode rows that share prefixes (no counterpart in vm_c): group j is the rows
+    // prefix_group_starts[j] .. prefix_group_starts[j + 1] - 1, whose first
+    // shared_prefix_lens[j] tokens lie in the blocks of its first row.  0 groups:
+    // every row reads its own.
+    const int32_t* prefix_group_starts = nullptr;  // device [num_prefix_groups + 1]
+    const int32_t* shared_prefix_lens = nullptr;   // device [num_prefix_groups]
+    int num_prefix_groups = 0;
 };
 
 class KVCacheManager;
@@ -68,12 +75,23 @@ struct HostBatchMetadata {
     int num_decodes = 0;
     int num_decode_tokens = 0;
     int num_computed_tokens = 0;  // cached-prefix tokens of the prefill requests
+    std::vector<int32_t> prefix_group_starts;  // of group_shared_prefixes; empty: no groups
+    std::vector<int32_t> shared_prefix_lens;
     bool ok = true;  // false if the block manager could not allocate
 };
 
 HostBatchMetadata build_batch_metadata(KVCacheManager& mgr,
                                        const std::vector<ScheduledRequest>& reqs,
                                        int kv_lookahead_tokens = 0);
+
+// Groups consecutive rows of a decode batch that begin with the same whole blocks, as
+// prefix caching leaves them, for one read of those blocks a group
+// (paged_attention_shared_prefix): fills prefix_group_starts and
+// shared_prefix_lens, or leaves them empty where a batch with prefill rows, or one
+// that would save fewer than min_saved_tokens reads of a token, gains nothing.
+// Row order is the batch's: rows of one prefix have to be neighbours.  Returns the
+// reads of a token that the groups save.
+int64_t group_shared_prefixes(HostBatchMetadata& h, int block_size, int64_t min_saved_tokens = 0);
 
 // Device buffers for one step's metadata, sized once for the largest batch.
 class DeviceBatchMetadata {
@@ -94,6 +112,8 @@ private:
     int64_t* slot_mapping_ = nullptr;
     int32_t* token_to_seq_ = nullptr;
     int32_t* token_positions_ = nullptr;
+    int32_t* prefix_group_starts_ = nullptr;
+    int32_t* shared_prefix_lens_ = nullptr;
 };
 
 }  // namespace vm_c

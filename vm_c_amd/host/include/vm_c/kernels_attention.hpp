@@ -131,4 +131,43 @@ void flash_attention_prefill_local_with_cache(
     int64_t block_size, const std::string& kv_cache_dtype, const std::string& layout,
     hipStream_t stream = nullptr);
 
+// Paged decode whose rows share prefixes (vmc_paged_attention_shared_prefix; no
+// counterpart in the reference): group j is the rows group_starts[j] ..
+// group_starts[j + 1] - 1, whose first shared_lens[j] tokens are read once,
+// through the table row of its first row.  Device arrays; workspace of the size
+// below or more.
+size_t paged_attention_shared_prefix_workspace_size(const AttentionParams& params, int num_groups);
+
+void paged_attention_shared_prefix(void* out, void* workspace, size_t workspace_bytes, const void* query,
+                                   const void* key_cache, const void* value_cache, const AttentionParams& params,
+                                   const int32_t* block_tables, const int32_t* seq_lens, const int32_t* group_starts,
+                                   const int32_t* shared_lens, int num_groups, const std::string& kv_cache_dtype,
+                                   hipStream_t stream = nullptr, const std::string& layout = "nhd");
+
+// Decoder tokens over an encoder's states (vmc_cross_attention; no counterpart in the
+// reference, whose models are decoders).  Strides in values; 0: contiguous [tokens]
+// [heads][head_dim].
+struct CrossAttentionParams {
+    int num_tokens = 0;
+    int num_keys = 0;
+    int num_seqs = 0;
+    int num_heads = 0;
+    int num_kv_heads = 0;
+    int head_dim = 0;
+    int64_t query_token_stride = 0;
+    int64_t query_head_stride = 0;
+    int64_t key_token_stride = 0;
+    int64_t key_head_stride = 0;
+    int64_t value_token_stride = 0;
+    int64_t value_head_stride = 0;
+    float scale = 1.0f;
+    ScalarType dtype = ScalarType::FLOAT16;
+};
+
+size_t cross_attention_workspace_size(const CrossAttentionParams& params);
+
+void cross_attention(void* out, void* workspace, size_t workspace_bytes, const void* query, const void* key,
+                     const void* value, const CrossAttentionParams& params, const int32_t* query_starts,
+                     const int32_t* key_starts, const int32_t* key_lens, hipStream_t stream = nullptr);
+
 }  // namespace vm_c

@@ -49,4 +49,16 @@ void fused_qk_norm_rope(void* q_buf, void* k_buf, const void* q_norm_weight,
                         int num_kv_heads, int head_dim, float rms_norm_eps, bool is_neox,
                         hipStream_t stream = nullptr, ScalarType dtype = ScalarType::FLOAT16);
 
+// RoPE and append from the fused QKV projection in one launch (vmc_rope_and_cache; no
+// counterpart in the reference): Q rotated into query_out, K rotated into the
+// pages at slot_mapping and / or key_out, V into the pages; fp32 table of
+// max_position rows of rotary_dim values, token strides in values (0: contiguous).
+void rope_and_cache(void* query_out, void* key_out, const void* query, const void* key, const void* value,
+                    const float* cos_sin, const int64_t* position_ids, void* key_cache, void* value_cache,
+                    const int64_t* slot_mapping, int num_tokens, int num_heads, int num_kv_heads, int head_dim,
+                    int rotary_dim, int64_t max_position, int64_t query_token_stride, int64_t key_token_stride,
+                    int64_t value_token_stride, bool is_neox, int64_t block_size, int64_t cache_stride,
+                    const std::string& kv_cache_dtype, hipStream_t stream = nullptr,
+                    ScalarType dtype = ScalarType::FLOAT16, const std::string& layout = "nhd");
+
 }  // namespace vm_c

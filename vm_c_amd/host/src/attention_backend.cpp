@@ -2,6 +2,8 @@
 // (vm_c src/model/attention_backend.cpp:15-238) over the gfx950 kernels.
 #include "vm_c/attention_backend.hpp"
 
+#include <algorithm>
+
 namespace vm_c {
 
 namespace {
@@ -72,7 +74,8 @@ void PagedAttentionBackend::forward_prefill(void* output, const void* query, con
                                   head_dim, scale, meta.token_to_seq, meta.token_positions, dtype, stream);
 }
 
-// attention_backend.cpp:67-99: one query row per request
+// attention_backend.cpp:67-99: one query row per request; rows that share prefixes
+// (no counterpart in the reference) read those once a group
 void PagedAttentionBackend::forward_decode(void* output, const void* query, const void* key_cache,
                                            const void* value_cache, const AttentionMetadata& meta,
                                            int num_heads, int num_kv_heads, int head_dim, float scale,
@@ -88,6 +91,16 @@ void PagedAttentionBackend::forward_decode(void* output, const void* query, cons
     p.max_seq_len = meta.max_num_blocks_per_req * (int)block_size;
     p.scale = scale;
     p.dtype = dtype;
+    if (meta.num_prefix_groups > 0) {
+        // (where the workspace was made for fewer rows, each row reads its own, as below)
+        const size_t shared = paged_attention_shared_prefix_workspace_size(p, meta.num_prefix_groups);
+        if (ws_ && shared > 0 && shared <= ws_bytes_) {
+            paged_attention_shared_prefix(output, ws_, ws_bytes_, query, key_cache, value_cache, p, meta.block_tables,
+                                          meta.seq_lens, meta.prefix_group_starts, meta.shared_prefix_lens,
+                                          meta.num_prefix_groups, kv_cache_dtype_, stream, kv_cache_layout_);
+            return;
+        }
+    }
     const size_t need = paged_attention_v2_workspace_size(p);
     if (ws_ && need <= ws_bytes_) {
         paged_attention_v2(output, nullptr, nullptr, ws_, query, key_cache, value_cache, p,
@@ -101,15 +114,18 @@ void PagedAttentionBackend::forward_decode(void* output, const void* query, cons
 
 // pre-sizes the split workspace for max_num_seqs requests of up to 32768
 // tokens (a batch that needs more runs one pass per request, without it),
+// the shared-prefix decode's for as many requests and groups,
 // and the local prefill's V^T tiles for max_num_batched_tokens tokens (the
 // same buffer: prefill and decode calls are ordered on the stream)
 void PagedAttentionBackend::ensure_workspace(int max_num_batched_tokens, int max_num_seqs,
                                              int num_attention_heads, int num_kv_heads,
                                              int head_dim, int gpu_device) {
-    const size_t need = std::max(vmc_paged_decode_workspace_size(max_num_seqs, num_attention_heads, num_kv_heads,
-                                                                 head_dim, 32768 / 16, 16, 0),
-                                 vmc_flash_attention_prefill_workspace_size(max_num_batched_tokens, num_kv_heads,
-                                                                            head_dim));
+    const size_t need =
+        std::max({vmc_paged_decode_workspace_size(max_num_seqs, num_attention_heads, num_kv_heads, head_dim, 32768 / 16,
+                                                  16, 0),
+                  vmc_shared_prefix_workspace_size(max_num_seqs, num_attention_heads, num_kv_heads, head_dim,
+                                                   max_num_seqs),
+                  vmc_flash_attention_prefill_workspace_size(max_num_batched_tokens, num_kv_heads, head_dim)});
     if (need <= ws_bytes_) return;
     HIP_CHECK(hipSetDevice(gpu_device));
     if (ws_) HIP_CHECK(hipFree(ws_));

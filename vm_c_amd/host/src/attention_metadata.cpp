@@ -59,6 +59,43 @@ HostBatchMetadata build_batch_metadata(KVCacheManager& mgr, const std::vector<Sc
     return h;
 }
 
+int64_t group_shared_prefixes(HostBatchMetadata& h, int block_size, int64_t min_saved_tokens) {
+    h.prefix_group_starts.clear();
+    h.shared_prefix_lens.clear();
+    if (block_size <= 0) throw std::runtime_error("group_shared_prefixes: block_size must be positive");
+    if (h.num_prefills > 0 || h.num_reqs < 2) return 0;
+    const int mb = h.max_num_blocks_per_req;
+    // whole blocks that rows a and b begin with, at most n
+    auto common = [&](int a, int b, int n) {
+        n = std::min({n, h.seq_lens[a] / block_size, h.seq_lens[b] / block_size, mb});
+        const int32_t *x = &h.block_tables[(size_t)a * mb], *y = &h.block_tables[(size_t)b * mb];
+        int c = 0;
+        while (c < n && x[c] == y[c] && x[c] >= 0) ++c;
+        return c;
+    };
+    int64_t saved = 0;
+    std::vector<int32_t> starts, lens;
+    for (int first = 0; first < h.num_reqs;) {
+        int rows = 1, blocks = 0;
+        while (first + rows < h.num_reqs) {
+            // one more row, if the group then saves no less than without it
+            const int c = common(first, first + rows, rows == 1 ? mb : blocks);
+            if (c == 0 || (int64_t)rows * c < (int64_t)(rows - 1) * blocks) break;
+            blocks = c;
+            ++rows;
+        }
+        starts.push_back(first);
+        lens.push_back(blocks * block_size);
+        saved += (int64_t)(rows - 1) * blocks * block_size;
+        first += rows;
+    }
+    if (saved == 0 || saved < min_saved_tokens) return 0;
+    starts.push_back(h.num_reqs);
+    h.prefix_group_starts = std::move(starts);
+    h.shared_prefix_lens = std::move(lens);
+    return saved;
+}
+
 DeviceBatchMetadata::DeviceBatchMetadata(int max_num_reqs, int max_num_tokens, int max_num_blocks_per_req)
     : max_reqs_(max_num_reqs), max_tokens_(max_num_tokens), max_blocks_(max_num_blocks_per_req) {
     HIP_CHECK(hipMalloc(&block_tables_, sizeof(int32_t) * std::max(1, max_reqs_ * max_blocks_)));
@@ -66,11 +103,13 @@ DeviceBatchMetadata::DeviceBatchMetadata(int max_num_reqs, int max_num_tokens, i
     HIP_CHECK(hipMalloc(&slot_mapping_, sizeof(int64_t) * std::max(1, max_tokens_)));
     HIP_CHECK(hipMalloc(&token_to_seq_, sizeof(int32_t) * std::max(1, max_tokens_)));
     HIP_CHECK(hipMalloc(&token_positions_, sizeof(int32_t) * std::max(1, max_tokens_)));
+    HIP_CHECK(hipMalloc(&prefix_group_starts_, sizeof(int32_t) * (std::max(0, max_reqs_) + 1)));
+    HIP_CHECK(hipMalloc(&shared_prefix_lens_, sizeof(int32_t) * std::max(1, max_reqs_)));
 }
 
 DeviceBatchMetadata::~DeviceBatchMetadata() {
     for (void* p : {(void*)block_tables_, (void*)seq_lens_, (void*)slot_mapping_, (void*)token_to_seq_,
-                    (void*)token_positions_})
+                    (void*)token_positions_, (void*)prefix_group_starts_, (void*)shared_prefix_lens_})
         if (p) (void)hipFree(p);
 }
 
@@ -87,7 +126,19 @@ AttentionMetadata DeviceBatchMetadata::upload(const HostBatchMetadata& h, int bl
         cp(token_to_seq_, h.token_to_seq.data(), h.token_to_seq.size() * sizeof(int32_t));
         cp(token_positions_, h.token_positions.data(), h.token_positions.size() * sizeof(int32_t));
     }
+    const size_t groups = h.shared_prefix_lens.size();
+    if (groups > 0) {
+        if (groups > (size_t)h.num_reqs || h.prefix_group_starts.size() != groups + 1)
+            throw std::runtime_error("DeviceBatchMetadata: prefix groups and their starts disagree");
+        cp(prefix_group_starts_, h.prefix_group_starts.data(), (groups + 1) * sizeof(int32_t));
+        cp(shared_prefix_lens_, h.shared_prefix_lens.data(), groups * sizeof(int32_t));
+    }
     AttentionMetadata m;
+    if (groups > 0) {
+        m.prefix_group_starts = prefix_group_starts_;
+        m.shared_prefix_lens = shared_prefix_lens_;
+        m.num_prefix_groups = (int)groups;
+    }
     m.block_tables = h.max_num_blocks_per_req > 0 ? block_tables_ : nullptr;
     m.seq_lens = seq_lens_;
     m.slot_mapping = slot_mapping_;

@@ -354,6 +354,40 @@ void paged_attention_v2(void* out, void* exp_sums, void* max_logits, void* tmp_o
                                         paged_attention_v2_workspace_size(p), stream));
 }
 
+size_t paged_attention_shared_prefix_workspace_size(const AttentionParams& p, int num_groups) {
+    return vmc_shared_prefix_workspace_size(p.batch_size, p.num_heads, p.num_kv_heads, p.head_dim, num_groups);
+}
+
+void paged_attention_shared_prefix(void* out, void* workspace, size_t workspace_bytes, const void* query,
+                                   const void* key_cache, const void* value_cache, const AttentionParams& p,
+                                   const int32_t* block_tables, const int32_t* seq_lens, const int32_t* group_starts,
+                                   const int32_t* shared_lens, int num_groups, const std::string& kv_cache_dtype,
+                                   hipStream_t stream, const std::string& layout) {
+    check_params(p, nullptr);
+    VMC_CALL(vmc_paged_attention_shared_prefix(out, query, key_cache, value_cache, block_tables, seq_lens, group_starts,
+                                               shared_lens, p.batch_size, num_groups, p.num_heads, p.num_kv_heads,
+                                               p.head_dim, p.block_size, p.max_num_blocks_per_req, p.scale,
+                                               vmc_dtype_of(p.dtype), vmc_kv_format_of(kv_cache_dtype, p.dtype),
+                                               vmc_layout_of(layout), workspace, workspace_bytes, stream));
+}
+
+size_t cross_attention_workspace_size(const CrossAttentionParams& p) {
+    return vmc_cross_attention_workspace_size(p.num_tokens, p.num_seqs, p.num_heads, p.num_kv_heads, p.head_dim);
+}
+
+void cross_attention(void* out, void* workspace, size_t workspace_bytes, const void* query, const void* key,
+                     const void* value, const CrossAttentionParams& p, const int32_t* query_starts,
+                     const int32_t* key_starts, const int32_t* key_lens, hipStream_t stream) {
+    const int64_t d = p.head_dim, qt = (int64_t)p.num_heads * d, kt = (int64_t)p.num_kv_heads * d;
+    auto or_else = [](int64_t stride, int64_t contiguous) { return stride != 0 ? stride : contiguous; };
+    VMC_CALL(vmc_cross_attention(out, query, key, value, query_starts, key_starts, key_lens, p.num_tokens, p.num_keys,
+                                 p.num_seqs, p.num_heads, p.num_kv_heads, p.head_dim, or_else(p.query_token_stride, qt),
+                                 or_else(p.query_head_stride, d), or_else(p.key_token_stride, kt),
+                                 or_else(p.key_head_stride, d), or_else(p.value_token_stride, kt),
+                                 or_else(p.value_head_stride, d), p.scale, vmc_dtype_of(p.dtype), workspace,
+                                 workspace_bytes, stream));
+}
+
 // ------------------------------------------------------------ prefill
 
 void flash_attention_prefill_local(void* output, const void* query, const void* key,
@@ -428,6 +462,23 @@ void fused_qk_norm_rope(void* q_buf, void* k_buf, const void* q_norm_weight,
                                           num_tokens, num_heads, num_kv_heads, head_dim,
                                           rms_norm_eps, is_neox ? 1 : 0, 0, 0, VMC_KV_F16,
                                           VMC_LAYOUT_NHD, nullptr, vmc_dtype_of(dtype), stream));
+}
+
+void rope_and_cache(void* query_out, void* key_out, const void* query, const void* key, const void* value,
+                    const float* cos_sin, const int64_t* position_ids, void* key_cache, void* value_cache,
+                    const int64_t* slot_mapping, int num_tokens, int num_heads, int num_kv_heads, int head_dim,
+                    int rotary_dim, int64_t max_position, int64_t query_token_stride, int64_t key_token_stride,
+                    int64_t value_token_stride, bool is_neox, int64_t block_size, int64_t cache_stride,
+                    const std::string& kv_cache_dtype, hipStream_t stream, ScalarType dtype,
+                    const std::string& layout) {
+    const int64_t qt = (int64_t)num_heads * head_dim, kt = (int64_t)num_kv_heads * head_dim;
+    VMC_CALL(vmc_rope_and_cache(query_out, key_out, query, key, value, cos_sin, position_ids, key_cache, value_cache,
+                                slot_mapping, num_tokens, num_heads, num_kv_heads, head_dim, rotary_dim, max_position,
+                                query_token_stride != 0 ? query_token_stride : qt,
+                                key_token_stride != 0 ? key_token_stride : kt,
+                                value_token_stride != 0 ? value_token_stride : kt, is_neox ? 1 : 0, block_size,
+                                cache_stride, vmc_kv_format_of(kv_cache_dtype, dtype), vmc_layout_of(layout),
+                                vmc_dtype_of(dtype), stream));
 }
 
 }  // namespace vm_c
