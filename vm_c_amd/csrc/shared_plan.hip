@@ -28,7 +28,7 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(PlanParams p)
     const PlanSums x = plan_sets(p, lds, s_desc, i);
     plan_out(p, x, s_desc, lds.cum, i);
     if (p.whole) return;
-    const int n = plan_ranges(x.total, p.grid, p.umin);
+    const int n = plan_ranges(x.total, p.grid, p.cus);
     RangeRec r = {};
     if (i < n) {
         r.ntiles = range_begin(lds, s_desc, p.nsets, (int)div_floor<long long>((long long)i * x.total, n), r);
@@ -84,7 +84,7 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_long_kernel(PlanPara
     if (tid == 0) p.cum[p.nsets] = total;
     if (p.whole) return;
     __syncthreads();
-    const int n = plan_ranges(total, p.grid, p.umin);
+    const int n = plan_ranges(total, p.grid, p.cus);
     for (int w = tid; w < p.grid; w += nt) {
         RangeRec r = {}, e = {};
         if (w < n) {
@@ -166,7 +166,7 @@ __global__ void __launch_bounds__(256) shared_merge_paged_kernel(TileParams p, i
     const int b = blockIdx.x / p.Hq, hq = blockIdx.x % p.Hq, g = hq / p.G;
     const int64_t total = p.cum[p.nsets];
     const RowRec rec = p.row[b];
-    const int n = plan_ranges(total, p.grid, p.umin);
+    const int n = plan_ranges(total, p.grid, p.cus);
     int w0[2] = {0, 0}, cnt[2] = {0, 0};  // first range and pieces: common keys, own keys
     int64_t base[2] = {0, 0};             // partial row of range 0
     if (rec.grp_tiles) {
@@ -234,7 +234,7 @@ __global__ void __launch_bounds__(256) shared_merge_local_kernel(TileParams p, i
     if (rec.t == 0 || (me.set == rec.set && me.g == rec.g && me.rb == rec.rb && me.t > 0)) return;
     const int lane = threadIdx.x % LR, nrow = min(RB, rec.d.ntok * p.G - RB * rec.rb);
     const int64_t total = p.cum[p.nsets];
-    const int n = plan_ranges(total, p.grid, p.umin);
+    const int n = plan_ranges(total, p.grid, p.cus);
     const int64_t last = p.cum[rec.set] + ((int64_t)rec.g * rec.d.nb + rec.rb + 1) * (rec.d.tiles + kItemCost) - 1;
     const int cnt = plan_range_of(last, total, n) - w + 1;
     for (int r = NG * blockIdx.y + threadIdx.x / LR; r < nrow; r += NG * gridDim.y) {
@@ -349,7 +349,7 @@ int shared_tiles(const SharedArgs& a, void* ws, hipStream_t s) {
     pl.range = reinterpret_cast<RangeRec*>(w + sh.range);
     pl.row = reinterpret_cast<RowRec*>(w + sh.row);
     pl.grid = sh.grid;
-    pl.umin = kUnitsMin;
+    pl.cus = num_cus();
     pl.gs = reinterpret_cast<int32_t*>(w + sh.gs);
     // units fit 32 bits where even the longest sets that fit the call do
     const int64_t tiles = paged ? pl.max_keys / 64 + 2 : a.num_keys / 64 + 2;
@@ -386,7 +386,7 @@ int shared_tiles(const SharedArgs& a, void* ws, hipStream_t s) {
     p.whole = sh.whole;
     p.total_rows = a.rows;
     p.grid = sh.grid;
-    p.umin = kUnitsMin;
+    p.cus = pl.cus;
     p.part = reinterpret_cast<float*>(w + sh.part);
     if (paged) {
         p.kp = a.kp;

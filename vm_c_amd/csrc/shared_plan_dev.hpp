@@ -8,8 +8,6 @@
 namespace vmc {
 namespace {
 
-constexpr int kUnitsMin = kItemCost + 1;  // fewest units of a range: one tile
-
 // Inclusive scan over the wave in six DPP steps (row_shr 1, 2, 4, 8, then the last lane of
 // the row before, then lane 31); op(v, 0) = v for the values scanned
 template <typename Op>

@@ -221,13 +221,12 @@ __global__ void __launch_bounds__(256, tile_per_cu(D)) shared_tile_kernel(TilePa
     } else if (p.fused) {
         const PlanSums sums = plan_sets(p.plan, plan, lds.desc, tid);
         if (blockIdx.x == 0) plan_out(p.plan, sums, lds.desc, plan.cum, tid);
-        RangeRec r = {}, e;
-        const int n = plan_ranges(sums.total, p.grid, p.umin);
-        if (range < n) {
-            const int u0 = (int)div_floor<long long>((long long)range * sums.total, n);
-            const int u1 = (int)div_floor<long long>((long long)(range + 1) * sums.total, n);
-            r.ntiles = (u1 < sums.total ? range_begin(plan, lds.desc, p.nsets, u1, e) : sums.total_t);
-            r.ntiles -= range_begin(plan, lds.desc, p.nsets, u0, r);
+        RangeRec r = {};
+        const int n = plan_ranges(sums.total, p.grid, p.cus);
+        if (range < n) {  // even lanes: where the range begins, odd ones: where the next does
+            const int u = (int)div_floor<long long>((long long)(range + (lane & 1)) * sums.total, n);
+            const int before = u < sums.total ? range_begin(plan, lds.desc, p.nsets, u, r) : sums.total_t;
+            r.ntiles = __builtin_amdgcn_readlane(before, 1) - __builtin_amdgcn_readlane(before, 0);
         }
         if (tid == 0 && !p.paged) const_cast<RangeRec*>(p.range)[range] = r;  // (the merge's)
         cc.set = __builtin_amdgcn_readfirstlane(r.set);
