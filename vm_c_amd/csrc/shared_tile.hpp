@@ -324,8 +324,8 @@ __global__ void __launch_bounds__(256, tile_per_cu(D)) shared_tile_kernel(TilePa
     auto part_row = [&](int i) __attribute__((always_inline)) { return kBN / W * w + TR * i + lane_row; };
     auto part_col = [&](int i) __attribute__((always_inline)) { return lane_col ^ (16u * (uint32_t)tile_swz<D>(TR * i)); };
     // (paged: of the row in its 16-key chunk, the same for K and V)
-    const uint32_t off_k = (uint32_t)part_row(0) % (SRC == TS_LOCAL ? kBN : 16) * (uint32_t)p.k_row;
-    const uint32_t off_v = SRC == TS_LOCAL ? (uint32_t)part_row(0) * (uint32_t)p.v_row : off_k;
+    uint32_t off_k = (uint32_t)part_row(0) % (SRC == TS_LOCAL ? kBN : 16) * (uint32_t)p.k_row;
+    uint32_t off_v = SRC == TS_LOCAL ? (uint32_t)part_row(0) * (uint32_t)p.v_row : off_k;
     // this wave's part of K or V of a tile into LDS at dst
     auto transfer = [&](bool is_v, const Rec& x, uint32_t dst) __attribute__((always_inline)) {
         const uint64_t b64 = (uint64_t)(is_v ? p.vp + (SRC == TS_LOCAL ? x.v : x.k[0]) : p.kp + x.k[0]);
@@ -337,7 +337,7 @@ __global__ void __launch_bounds__(256, tile_per_cu(D)) shared_tile_kernel(TilePa
         // opaque, or the compiler computes every transfer's offset ahead, and where those fill
         // the registers (head_dim 256) reads them from memory between transfers, behind a
         // wait for all of them
-        if constexpr (D == 256) asm volatile("" : "+v"(lane_row), "+v"(lane_col));
+        if constexpr (D == 256) asm volatile("" : "+v"(lane_row), "+v"(lane_col), "+v"(off_k), "+v"(off_v));
         if (x.first == 0 && x.last >= kBN - 1) {
 #pragma unroll
             for (int i = 0; i < NTR; ++i)
@@ -589,30 +589,23 @@ __global__ void __launch_bounds__(256, tile_per_cu(D)) shared_tile_kernel(TilePa
             for (int b = 0; b < HB; ++b)
 #pragma unroll
                 for (int j = 0; j < 16; ++j) mloc = fmaxf(mloc, sacc[b][j]);
-            if (__ballot(mloc * csc > m_thr)) {  // rare after the first tiles
+            float top = v_base;  // kConv: of the largest values so far
+            if constexpr (kConv) top = fmaxf(top, fmaxf(fmaxf(vexp[0], vexp[1]), fmaxf(vexp[2], vexp[3])));
+            if (__ballot(mloc * csc > m_thr || top > v_base)) {  // rare after the first tiles
                 const float mrow = fmaxf(mloc, shfl_xor(mloc, 32)) * csc;
                 const bool upd = mrow > m_thr;  // the same in both halves of the row
-                const float alpha = upd ? __builtin_amdgcn_exp2f(m_run - mrow) : 1.0f;  // 0 from -inf
+                float alpha = upd ? __builtin_amdgcn_exp2f(m_run - mrow) : 1.0f;  // 0 from -inf
                 m_run = upd ? mrow : m_run;
                 m_thr = m_run + 8.0f;
                 l_part *= alpha;
+                if constexpr (kConv) alpha *= __builtin_amdgcn_exp2f(v_base - top);  // 0 from -inf
+                v_base = top;
 #pragma unroll
                 for (int m = 0; m < D / 32; ++m)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) o[m][i] *= alpha;
             }
             const float ref = m_run == -__builtin_inff() ? 0.0f : m_run - kOff;
-            if constexpr (kConv) {
-                const float top = fmaxf(fmaxf(vexp[0], vexp[1]), fmaxf(vexp[2], vexp[3]));
-                if (__builtin_amdgcn_readfirstlane(top > v_base)) {  // larger values than so far
-                    const float alpha = __builtin_amdgcn_exp2f(v_base - top);  // 0 from -inf
-                    v_base = top;
-#pragma unroll
-                    for (int m = 0; m < D / 32; ++m)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) o[m][i] *= alpha;
-                }
-            }
             u32x4 pt[2][2 * HB];  // [term][16-key chunk]
             float sum = 0.0f;
 #pragma unroll
