@@ -278,7 +278,6 @@ int launch_merge(const TileParams& p, int D, bool bf, int RB, hipStream_t s) {
 // How a call runs, from its sizes alone (lengths are on the device).
 struct Shape {
     int whole, grid;  // one item a workgroup; ranges (whole: workgroups)
-    bool conv;        // bf16 V is converted to fp16
     size_t cum, cumt, desc, range, row, gs, part, bytes;  // workspace offsets, size
 };
 
@@ -286,13 +285,14 @@ Shape shape_of(bool paged, int rows, int nsets, int Hq, int Hkv, int D) {
     Shape sh = {};
     const int64_t G = Hq / Hkv, sets = std::max(nsets, 1);
     sh.grid = num_cus() * tile_per_cu(D);
-    // Whole items where sets of many rows give several times the workgroups
+    // Whole items where sets of many rows give several times the workgroups: 8 x 1024 rows over
+    // 2048 states take 459 us with the plan, 503 as ranges with the merge; with fewer items
+    // the last workgroups' share shows
     const int64_t items = (int64_t)Hkv * (rows * G / kTileRows + std::min<int64_t>(rows, sets));
     if (!paged && rows * G >= kTileRows * sets && items >= 4 * (int64_t)sh.grid && items < (1 << 24)) {
         sh.whole = 1;
         sh.grid = (int)((items + 7) & ~7);
     }
-    sh.conv = rows * G >= 64 * sets;
     const int64_t total = paged ? (int64_t)nsets + rows : nsets;
     const int64_t prow = sh.whole ? 0 : paged ? (int64_t)sh.grid * kTileRows + 2 * (int64_t)rows * Hq : 2 * (int64_t)sh.grid * kTileRows;
     auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
@@ -408,9 +408,9 @@ int shared_tiles(const SharedArgs& a, void* ws, hipStream_t s) {
     }
     const int src = !paged ? 0 : a.src == GEN_Q8 ? 2 : a.src == GEN_Q4 ? 3 : 1;
     const bool bf = a.q_bf16 != 0;
-    const int rc = a.D == 64    ? shared_tile_d64(p, src, bf, sh.conv, sh.grid, s)
-                   : a.D == 128 ? shared_tile_d128(p, src, bf, sh.conv, sh.grid, s)
-                                : shared_tile_d256(p, src, bf, sh.conv, sh.grid, s);
+    const int rc = a.D == 64    ? shared_tile_d64(p, src, bf, sh.grid, s)
+                   : a.D == 128 ? shared_tile_d128(p, src, bf, sh.grid, s)
+                                : shared_tile_d256(p, src, bf, sh.grid, s);
     if (rc != VMC_OK || sh.whole) return rc;
     return launch_merge(p, a.D, bf, pl.RB, s);
 }

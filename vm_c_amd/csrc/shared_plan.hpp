@@ -39,13 +39,15 @@ struct RowRec {
 
 // An item's first kItemCost units stand for what a workgroup spends on the item beside
 // its tiles (the next rows' Q, the last rows' partial results), so that a range of
-// short items gets fewer tiles.
+// short items gets fewer tiles.  2: 64 rows over 32768 common and 32 to 2048 own tokens
+// take 96.7 us, 101.5 with 1; 24 ragged targets 39.0, 38.1 with 1.
 constexpr int kItemCost = 2;
 
 constexpr int kTileWaves = 4;  // waves of the shared-keys kernel, 32 rows each
 constexpr int kTileRows = 32 * kTileWaves;  // rows of an item (GGUF pages: half)
 // its workgroups that fit a CU: 64 KB of tiles (head_dim 64: 48, 256: 128), 168 registers a
-// lane at head_dim 64, 256 at 128, 512 at 256
+// lane at head_dim 64 (two workgroups there: 43 instead of 35 us, the kernel alone, for 48
+// rows with 64 to 4096 tokens of their own), 256 at 128, 512 at 256
 __host__ __device__ constexpr int tile_per_cu(int D) { return D == 64 ? 3 : D == 128 ? 2 : 1; }
 
 // Sets of a call whose plan every workgroup of the shared-keys kernel makes for itself, in
@@ -98,9 +100,9 @@ struct TileParams {
     const int32_t* seq_lens;
 };
 
-int shared_tile_d64(const TileParams& p, int src, bool q_bf16, bool conv, unsigned grid, hipStream_t s);
-int shared_tile_d128(const TileParams& p, int src, bool q_bf16, bool conv, unsigned grid, hipStream_t s);
-int shared_tile_d256(const TileParams& p, int src, bool q_bf16, bool conv, unsigned grid, hipStream_t s);
+int shared_tile_d64(const TileParams& p, int src, bool q_bf16, unsigned grid, hipStream_t s);
+int shared_tile_d128(const TileParams& p, int src, bool q_bf16, unsigned grid, hipStream_t s);
+int shared_tile_d256(const TileParams& p, int src, bool q_bf16, unsigned grid, hipStream_t s);
 
 // The MFMA path of a call: whether it takes the shape, what workspace it needs (its
 // sizes alone decide), and the launches.

@@ -8,12 +8,13 @@
 // pairs: a group of 64 sequences with G = 4 fills 256 rows, a single sequence
 // G of them.  Each workgroup takes one even range of the axis, whatever the
 // sets' lengths are, and streams its tiles through LDS without a stop between
-// items; a plan kernel turns the lengths into the axis (shared_plan.hip), and
-// pieces of items that a range cut meet in a merge kernel through fp32 partial
-// rows.  Where items are many times the workgroups (whole targets), each takes
-// one whole item instead, without partial rows and merge.
+// items; a plan turns the lengths into the axis (shared_plan.hpp), and pieces of
+// items that a range cut meet in a merge kernel through fp32 partial rows.
+// Where items are many times the workgroups (whole targets), each takes one
+// whole item instead, without partial rows and merge.
 //
-// What bounds it: HBM with few rows, the matrix cores with many.
+// What bounds it: HBM with few rows, with many the matrix cores together with the
+// vector instructions of the softmax, which a wave's products wait for.
 //   S^T[32 keys x 32 rows] = K . Q^T, O^T[D x 32 rows] += V^T . P^T on
 //   v_mfma_f32_32x32x16: a row is one lane column in both, so its running max,
 //   rescale and sums stay in the lane (and its partner 32 lanes on); V^T
@@ -21,22 +22,30 @@
 //   contraction index is permuted as P leaves the S registers (k = 8h + e <->
 //   key 16c + 8 (e / 4) + 4h + e % 4).
 //   A wave has 32 of the item's rows; waves beyond the rows only load.
+// Measured (with the plan and merge): 32 sequences of 5 tokens, 200 to 4096 states, 32
+// / 8 heads of 128, bf16: 47 us, 3.2 TB/s; 48 rows of head_dim 64 with 64 to 4096
+// tokens of their own: 44 us, 2.6 TB/s; 64 rows over 32768 common tokens and 32 to
+// 2048 own: 96 us, 2.7 TB/s and 0.36 PFLOP/s; 8 x 1024 rows over 2048 states: 360
+// us, 0.76 PFLOP/s (a large product of the library: 1.21); 4 rows over 512 common
+// tokens: 13.4 us, of which launch, plan and merge are 9.
+//
 // 16-bit rows arrive by load-to-LDS transfers, two or three tile slots; GGUF
 // blocks through registers, dequantized to fp16 (code * d rounded once: 2^-11
 // of a value at most) by two waves for the two that have rows.
 //
-// Weights enter P . V as fp16 where that costs nothing the result shows: two of them cut
-// to fp16 by one instruction, and summed as they were cut by another, so that the cut
-// (0 to 2^-10 of a weight) stays out of their mean, and 2^-11 of a value at most is
-// left, beside the 2^-8 of a bf16 result.  bf16 V becomes fp16 for it, by the waves that fetched its rows, while slower waves still multiply:
-// each 16 keys times 2^8 (values up to 255), 1 (larger ones) or 2^20 (all below
-// 2^-12), which their weights undo against the largest of an item's.  So values from
-// 2^-33 to 65504 keep their bits; the smaller ones of a chunk are cut, off by 2^-24
-// over its scale at most.  A chunk outside that range
-// makes its rows rerun.  Elsewhere (fp16 results; few rows, where the products
-// are not what counts) weights are two 16-bit terms of V's type, which leave
-// 2^-17 (bf16) or 2^-23 (fp16) of a weight: one term of 8 bits, or of the result's
-// own 11, would add as much error as the rounding of the result.
+// P . V runs in fp16.  A bf16 result takes weights of one fp16 term: two of them cut to
+// fp16 by one instruction, and summed as they were cut by another, so that the cut (0
+// to 2^-10 of a weight) stays out of their mean, and 2^-11 of a value at most is
+// left, beside the result's own 2^-8 (two bf16 terms and bf16 V: 495 instead of 453 us
+// for 8 x 1024 rows over 2048 states, the kernel alone, and no faster with few
+// rows).  An fp16 result takes two terms, which leave 2^-23 of a weight: one would add
+// as much error as the rounding of the result.
+// bf16 V becomes fp16 in LDS, by the waves that fetched its rows, while slower waves
+// still multiply: each 16 keys times 2^8 (values up to 255), 1 (larger ones) or
+// 2^20 (all below 2^-12), which their weights undo against the largest of an
+// item's.  So values from 2^-33 to 65504 keep their bits; the smaller ones of a
+// chunk are cut, off by 2^-24 over its scale at most.  A chunk outside that range
+// makes its rows rerun.
 #pragma once
 
 #include "generic_row.hpp"
@@ -49,13 +58,12 @@ namespace {
 
 constexpr int kBN = 64;  // keys per tile
 
-// two 16-bit terms of a pair of weights
-template <bool BF>
+// two fp16 terms of a pair of weights
 __device__ __forceinline__ void two_terms(float a, float b, uint32_t& hi, uint32_t& lo) {
-    hi = (uint32_t)f32_to_half<BF>(a) | ((uint32_t)f32_to_half<BF>(b) << 16);
-    a -= half_to_f32<BF>((uint16_t)(hi & 0xffffu));
-    b -= half_to_f32<BF>((uint16_t)(hi >> 16));
-    lo = (uint32_t)f32_to_half<BF>(a) | ((uint32_t)f32_to_half<BF>(b) << 16);
+    hi = (uint32_t)f32_to_half<false>(a) | ((uint32_t)f32_to_half<false>(b) << 16);
+    a -= half_to_f32<false>((uint16_t)(hi & 0xffffu));
+    b -= half_to_f32<false>((uint16_t)(hi >> 16));
+    lo = (uint32_t)f32_to_half<false>(a) | ((uint32_t)f32_to_half<false>(b) << 16);
 }
 
 // chunk swizzle of a tile row of 2 D bytes: 16-byte chunk ch of row r sits at
@@ -123,9 +131,9 @@ __device__ __noinline__ void shared_row_exact(const uint16_t* q, const uint8_t* 
     wave_sync();
 }
 
-// BF: the products' type (LOCAL and PAGED: the rows'; GGUF: fp16, BF false);
-// QBF: the type of q and out
-template <int D, int SRC, bool QBF, bool CONV>
+// QBF: the type of q and out (LOCAL and PAGED: of the rows too).  BF in it: K . Q runs in
+// bf16 (GGUF: K is fp16 in LDS, and a bf16 q becomes it)
+template <int D, int SRC, bool QBF>
 __global__ void __launch_bounds__(256, tile_per_cu(D)) shared_tile_kernel(TileParams p) {
     constexpr int W = kTileWaves;
     constexpr bool kGguf = SRC == TS_Q8 || SRC == TS_Q4;
@@ -137,11 +145,9 @@ __global__ void __launch_bounds__(256, tile_per_cu(D)) shared_tile_kernel(TilePa
     constexpr int NTR = TILE / (1024 * W);            // transfers per wave and tensor
     constexpr int CW = kGguf ? W / 2 : W;             // waves with rows; the others dequantize
     constexpr int RB = 32 * CW;                       // rows of an item
-    constexpr bool kConv = CONV;                      // bf16 V is converted to fp16
-    static_assert(!CONV || BF, "fp16 V needs no conversion");
-    constexpr bool PBF = BF && !kConv;                // the type of P . V
-    constexpr int NT = PBF || !QBF ? 2 : 1;           // terms of a weight
-    constexpr float kOff = PBF ? 0.0f : 7.0f;         // weights are 2^(s - m + kOff), at most 2^15
+    constexpr bool kConv = BF;                        // bf16 V is converted to fp16
+    constexpr int NT = QBF ? 1 : 2;                   // fp16 terms of a weight
+    constexpr float kOff = 7.0f;                      // weights are 2^(s - m + kOff), at most 2^15
     constexpr int HB = D == 256 ? 1 : 2;              // 32-key blocks per softmax round
     // GGUF: blocks per dequantizing lane and tile (K's then V's), dwords from a block's
     // 4-byte floor
@@ -624,7 +630,7 @@ __global__ void __launch_bounds__(256, tile_per_cu(D)) shared_tile_kernel(TilePa
                     } else {
                         part += x0 + x1;
                         uint32_t t0, t1;
-                        two_terms<PBF>(x0, x1, t0, t1);
+                        two_terms(x0, x1, t0, t1);
                         pt[0][c][e >> 1] = t0;
                         pt[1][c][e >> 1] = t1;
                     }
@@ -632,7 +638,7 @@ __global__ void __launch_bounds__(256, tile_per_cu(D)) shared_tile_kernel(TilePa
                 sum += kConv ? part * __builtin_amdgcn_exp2f(v_base - vexp[2 * HB * r + c]) : part;
             }
             // O^T += V^T P^T
-            using MP = MT<PBF>;
+            using MP = MT<false>;
             using VP = typename MP::v8;
             u32x2 va[VA + 1][2];
             auto read_v = [&](int i) __attribute__((always_inline)) {
@@ -852,22 +858,20 @@ __global__ void __launch_bounds__(256, tile_per_cu(D)) shared_tile_kernel(TilePa
     if (bad_seen) rerun(start, units);
 }
 
-template <int D, int SRC, bool QBF, bool CONV = false>
+template <int D, int SRC, bool QBF>
 int launch_tile(const TileParams& p, unsigned grid, hipStream_t s) {
-    hipLaunchKernelGGL((shared_tile_kernel<D, SRC, QBF, CONV>), dim3(grid), dim3(64 * kTileWaves), 0, s, p);
+    hipLaunchKernelGGL((shared_tile_kernel<D, SRC, QBF>), dim3(grid), dim3(64 * kTileWaves), 0, s, p);
     VMC_LAUNCH_CHECK();
     return VMC_OK;
 }
 
 template <int D>
-int dispatch_tile(const TileParams& p, int src, bool qbf, bool conv, unsigned grid, hipStream_t s) {
+int dispatch_tile(const TileParams& p, int src, bool qbf, unsigned grid, hipStream_t s) {
     switch (src) {
         case TS_LOCAL:
-            if (!qbf) return launch_tile<D, TS_LOCAL, false>(p, grid, s);
-            return conv ? launch_tile<D, TS_LOCAL, true, true>(p, grid, s) : launch_tile<D, TS_LOCAL, true>(p, grid, s);
+            return qbf ? launch_tile<D, TS_LOCAL, true>(p, grid, s) : launch_tile<D, TS_LOCAL, false>(p, grid, s);
         case TS_PAGED:
-            if (!qbf) return launch_tile<D, TS_PAGED, false>(p, grid, s);
-            return conv ? launch_tile<D, TS_PAGED, true, true>(p, grid, s) : launch_tile<D, TS_PAGED, true>(p, grid, s);
+            return qbf ? launch_tile<D, TS_PAGED, true>(p, grid, s) : launch_tile<D, TS_PAGED, false>(p, grid, s);
         case TS_Q8: return qbf ? launch_tile<D, TS_Q8, true>(p, grid, s) : launch_tile<D, TS_Q8, false>(p, grid, s);
         case TS_Q4: return qbf ? launch_tile<D, TS_Q4, true>(p, grid, s) : launch_tile<D, TS_Q4, false>(p, grid, s);
         default: return VMC_EINVAL;

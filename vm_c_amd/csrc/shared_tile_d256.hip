@@ -3,8 +3,8 @@
 
 namespace vmc {
 
-int shared_tile_d256(const TileParams& p, int src, bool q_bf16, bool conv, unsigned grid, hipStream_t s) {
-    return dispatch_tile<256>(p, src, q_bf16, conv, grid, s);
+int shared_tile_d256(const TileParams& p, int src, bool q_bf16, unsigned grid, hipStream_t s) {
+    return dispatch_tile<256>(p, src, q_bf16, grid, s);
 }
 
 }  // namespace vmc
