@@ -71,9 +71,9 @@ public:
                         int num_kv_heads, int head_dim, float scale, int64_t block_size,
                         ScalarType dtype, hipStream_t stream) override;
 
-    // split-KV and shared-prefix decode workspace, also the local prefill's V^T tiles
-    // (0 until ensure_workspace)
-    size_t workspace_size() const override { return ws_bytes_; }
+    // split-KV decode workspace, also the local prefill's V^T tiles, and the shared-prefix
+    // decode's (0 until ensure_workspace)
+    size_t workspace_size() const override { return ws_bytes_ + shared_ws_bytes_; }
     void ensure_workspace(int max_num_batched_tokens, int max_num_seqs, int num_attention_heads,
                           int num_kv_heads, int head_dim, int gpu_device) override;
 
@@ -83,6 +83,8 @@ private:
     ScalarType activation_dtype_;
     void* ws_ = nullptr;
     size_t ws_bytes_ = 0;
+    void* shared_ws_ = nullptr;  // of its own: what fits ws_ decides how other calls run
+    size_t shared_ws_bytes_ = 0;
     int max_num_seqs_ = 0, num_heads_ = 0;
 };
 

@@ -2,8 +2,6 @@
 // (vm_c src/model/attention_backend.cpp:15-238) over the gfx950 kernels.
 #include "vm_c/attention_backend.hpp"
 
-#include <algorithm>
-
 namespace vm_c {
 
 namespace {
@@ -29,6 +27,7 @@ PagedAttentionBackend::PagedAttentionBackend(const std::string& kv_cache_layout,
 
 PagedAttentionBackend::~PagedAttentionBackend() {
     if (ws_) (void)hipFree(ws_);
+    if (shared_ws_) (void)hipFree(shared_ws_);
 }
 
 // attention_backend.cpp:15-32 (the reference stores the activation type)
@@ -94,10 +93,11 @@ void PagedAttentionBackend::forward_decode(void* output, const void* query, cons
     if (meta.num_prefix_groups > 0) {
         // (where the workspace was made for fewer rows, each row reads its own, as below)
         const size_t shared = paged_attention_shared_prefix_workspace_size(p, meta.num_prefix_groups);
-        if (ws_ && shared > 0 && shared <= ws_bytes_) {
-            paged_attention_shared_prefix(output, ws_, ws_bytes_, query, key_cache, value_cache, p, meta.block_tables,
-                                          meta.seq_lens, meta.prefix_group_starts, meta.shared_prefix_lens,
-                                          meta.num_prefix_groups, kv_cache_dtype_, stream, kv_cache_layout_);
+        if (shared_ws_ && shared > 0 && shared <= shared_ws_bytes_) {
+            paged_attention_shared_prefix(output, shared_ws_, shared_ws_bytes_, query, key_cache, value_cache, p,
+                                          meta.block_tables, meta.seq_lens, meta.prefix_group_starts,
+                                          meta.shared_prefix_lens, meta.num_prefix_groups, kv_cache_dtype_, stream,
+                                          kv_cache_layout_);
             return;
         }
     }
@@ -114,18 +114,26 @@ void PagedAttentionBackend::forward_decode(void* output, const void* query, cons
 
 // pre-sizes the split workspace for max_num_seqs requests of up to 32768
 // tokens (a batch that needs more runs one pass per request, without it),
-// the shared-prefix decode's for as many requests and groups,
+// the shared-prefix decode's workspace for as many requests and groups,
 // and the local prefill's V^T tiles for max_num_batched_tokens tokens (the
 // same buffer: prefill and decode calls are ordered on the stream)
 void PagedAttentionBackend::ensure_workspace(int max_num_batched_tokens, int max_num_seqs,
                                              int num_attention_heads, int num_kv_heads,
                                              int head_dim, int gpu_device) {
-    const size_t need =
-        std::max({vmc_paged_decode_workspace_size(max_num_seqs, num_attention_heads, num_kv_heads, head_dim, 32768 / 16,
-                                                  16, 0),
-                  vmc_shared_prefix_workspace_size(max_num_seqs, num_attention_heads, num_kv_heads, head_dim,
-                                                   max_num_seqs),
-                  vmc_flash_attention_prefill_workspace_size(max_num_batched_tokens, num_kv_heads, head_dim)});
+    const size_t need = std::max(vmc_paged_decode_workspace_size(max_num_seqs, num_attention_heads, num_kv_heads,
+                                                                 head_dim, 32768 / 16, 16, 0),
+                                 vmc_flash_attention_prefill_workspace_size(max_num_batched_tokens, num_kv_heads,
+                                                                            head_dim));
+    const size_t shared =
+        vmc_shared_prefix_workspace_size(max_num_seqs, num_attention_heads, num_kv_heads, head_dim, max_num_seqs);
+    if (shared > shared_ws_bytes_) {
+        HIP_CHECK(hipSetDevice(gpu_device));
+        if (shared_ws_) HIP_CHECK(hipFree(shared_ws_));
+        shared_ws_ = nullptr;
+        shared_ws_bytes_ = 0;
+        HIP_CHECK(hipMalloc(&shared_ws_, shared));
+        shared_ws_bytes_ = shared;
+    }
     if (need <= ws_bytes_) return;
     HIP_CHECK(hipSetDevice(gpu_device));
     if (ws_) HIP_CHECK(hipFree(ws_));
