@@ -90,7 +90,11 @@ HostBatchMetadata build_batch_metadata(KVCacheManager& mgr,
 // shared_prefix_lens, or leaves them empty where a batch with prefill rows, or one
 // that would save fewer than min_saved_tokens reads of a token, gains nothing.
 // Row order is the batch's: rows of one prefix have to be neighbours.  Returns the
-// reads of a token that the groups save.
+// reads of a token that the groups save.  What they are worth, with 32 / 8 heads of
+// 128, bf16 pages, us a decode without and with groups: 8 rows of 1024 common tokens
+// (7168 saved) 15.1, 16.8; 8 of 4096 (28672) 22.9, 18.6; 32 of 256 (7936) 19.6, 22.7; 32
+// of 1024 (31744) 26.1, 25.8; 32 of 4096 56.0, 27.7; 64 of 32768 675, 95.  So
+// min_saved_tokens of 16384 to 32768 is about even there.
 int64_t group_shared_prefixes(HostBatchMetadata& h, int block_size, int64_t min_saved_tokens = 0);
 
 // Device buffers for one step's metadata, sized once for the largest batch.
