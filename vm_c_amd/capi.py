@@ -392,6 +392,15 @@ def _on_current_device(t, what):
         raise VmcError(f"{what}: tensors are on {t.device}, not on the current device")
 
 
+def _torch():
+    import torch
+    return torch
+
+
+def _int64_row(t, n):
+    return t.dtype == _torch().int64 and t.numel() == n and t.is_contiguous()
+
+
 def _token_stride(t, what):
     """Values between the tokens of t [T][heads][dim], whose heads lie together."""
     T, H, D = t.shape
@@ -408,32 +417,36 @@ def rope_and_cache(query, key, value, cos_sin, position_ids, key_cache=None, val
     tensors of their own; cos_sin float [max_position][rotary_dim].  Rotates Q
     into query_out (returned; allocated where it is None) and K into the paged
     cache and / or key_out; appends V beside K."""
-    import torch
     T, Hq, D = query.shape
     Hkv = key.shape[1]
+    dtype = query.dtype
     if key.shape != (T, Hkv, D) or (value is not None and value.shape != key.shape):
         raise VmcError("rope_and_cache: query, key and value disagree in tokens, heads or head_dim")
-    if key.dtype != query.dtype or (value is not None and value.dtype != query.dtype):
+    if key.dtype != dtype or (value is not None and value.dtype != dtype):
         raise VmcError("rope_and_cache: query, key and value have one dtype")
-    if cos_sin.dtype != torch.float32 or not cos_sin.is_contiguous():
+    max_position, rotary_dim = cos_sin.shape
+    if cos_sin.dtype != _torch().float32 or not cos_sin.is_contiguous():
         raise VmcError("rope_and_cache: cos_sin is a contiguous float32 table")
-    for name, idx in (("position_ids", position_ids), ("slot_mapping", slot_mapping)):
-        if idx is not None and (idx.dtype != torch.int64 or idx.numel() != T or not idx.is_contiguous()):
-            raise VmcError(f"rope_and_cache: {name} is contiguous int64 [{T}]")
-    strides = (_token_stride(query, "query"), _token_stride(key, "key"),
-               0 if value is None else _token_stride(value, "value"))
-    for o, like in ((query_out, query), (key_out, key)):
-        if o is not None and (o.shape != like.shape or o.dtype != like.dtype or not o.is_contiguous()):
-            raise VmcError("rope_and_cache: query_out and key_out are contiguous, of their input's shape and dtype")
+    if position_ids is None or not _int64_row(position_ids, T) or \
+            not (slot_mapping is None or _int64_row(slot_mapping, T)):
+        raise VmcError(f"rope_and_cache: position_ids and slot_mapping are contiguous int64 [{T}]")
+    if query_out is not None and (query_out.shape != query.shape or query_out.dtype != dtype or
+                                  not query_out.is_contiguous()):
+        raise VmcError("rope_and_cache: query_out is contiguous, of query's shape and dtype")
+    if key_out is not None and (key_out.shape != key.shape or key_out.dtype != dtype or not key_out.is_contiguous()):
+        raise VmcError("rope_and_cache: key_out is contiguous, of key's shape and dtype")
+    q_stride, k_stride = _token_stride(query, "query"), _token_stride(key, "key")
+    v_stride = 0 if value is None else _token_stride(value, "value")
     _on_current_device(query, "rope_and_cache")
     if query_out is None:
-        query_out = torch.empty((T, Hq, D), dtype=query.dtype, device=query.device)
+        query_out = _torch().empty((T, Hq, D), dtype=dtype, device=query.device)
         if stream is not None:
             query_out.record_stream(stream)
     rc = load().vmc_rope_and_cache(
-        _ptr(query_out), _ptr(key_out), _ptr(query), _ptr(key), _ptr(value), _ptr(cos_sin), _ptr(position_ids),
-        _ptr(key_cache), _ptr(value_cache), _ptr(slot_mapping), T, Hq, Hkv, D, cos_sin.shape[1], cos_sin.shape[0],
-        *strides, int(bool(is_neox)), block_size, cache_stride, kv_format, layout, _dtype_code(query), _stream(stream))
+        query_out.data_ptr(), _ptr(key_out), query.data_ptr(), key.data_ptr(), _ptr(value), cos_sin.data_ptr(),
+        position_ids.data_ptr(), _ptr(key_cache), _ptr(value_cache), _ptr(slot_mapping), T, Hq, Hkv, D, rotary_dim,
+        max_position, q_stride, k_stride, v_stride, 1 if is_neox else 0, block_size, cache_stride, kv_format, layout,
+        _dtype_code(query), _stream(stream))
     _check(rc, "vmc_rope_and_cache")
     return query_out
 
