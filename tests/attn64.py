@@ -37,10 +37,10 @@ def attend(q, k, v, scale, qt, e_k=0.0, e_v=0.0, mixed=False):
     # weights on their way into the products with V.  For a bf16 result one fp16 term,
     # cut: off by x_k in 0 .. 2^-10, in the sum of the weights too, so that
     # o moves by sum_k w_k x_k (v_k - o), where any constant may be taken off x
-    # (sum_k w_k (v_k - o) = 0): 2^-11 sum_k w_k |v_k - o| at most.  For
-    # an fp16 result (a bf16 one of few rows is no worse) two terms, and a sum of the
-    # weights as they were: a first bf16 term leaves 2^-8 and a second
-    # half a step of its own binade, 2^-17 of the weight
+    # (sum_k w_k (v_k - o) = 0): 2^-11 sum_k w_k |v_k - o| at most.  For an
+    # fp16 result two terms, and a sum of the weights as they were: two of 8 bits would
+    # leave 2^-17 of the weight, two of fp16 leave 2^-23 (and the end of fp16: weights
+    # of 2^-31 of the largest and less)
     ew = 2.0 ** -11 if qt == "bf16" else 2.0 ** -17
     av = w @ np.abs(v)
     err = (w * ds) @ (np.abs(v) + np.abs(o)) + es * (av + np.abs(o)) + (ew + e_v) * av
